@@ -68,7 +68,9 @@ enum {
  */
 enum {
     SMLA_LAYOUT_V32 = 0,
-    SMLA_LAYOUT_MODEL1 = 1
+    SMLA_LAYOUT_MODEL1 = 1,
+    SMLA_LAYOUT_BF16 = 2,    /* smla_append_kv and smla_paged_decode alone: rows of 576 bf16 values, V the first 512 of them */
+    SMLA_LAYOUT_F16 = 3      /* the same of fp16 values; queries and outputs are fp16 then */
 };
 #define SMLA_M1_D_QK 512
 #define SMLA_M1_ROW_BYTES 584
@@ -340,6 +342,59 @@ int smla_decode_splitkv_noalloc(const void* q, const void* kv, const int32_t* in
                                 int page_block_size, int64_t kv_block_stride_bytes, int num_sm_parts,
                                 const float* attn_sink, const int32_t* topk_length,
                                 int impl, int32_t* status, void* stream);
+
+/*
+ * New tokens' rows into a paged cache, rotated on the way, and the same tokens' queries.  No counterpart in the reference
+ * (the serving engine writes its cache; row formats as of smla_pack_kv and SMLA_LAYOUT_*).
+ *   kv_c       [num_tokens, 512] (448 for MODEL1), k_pe [num_tokens, 64]: bf16 (fp16 for SMLA_LAYOUT_F16); rows kv_c_stride /
+ *              k_pe_stride values apart
+ *   slots      [num_tokens] int32, or int64 where slots64: row slots[t] of the cache (page slots[t] / page_block_size) takes token
+ *              t; a slot outside [0, num_pages * page_block_size) leaves the cache as it is.  Slots differ from one another.
+ *   positions  [num_tokens] int32 or int64, rows of cos_sin [num_positions, 64] fp32 (32 cosines | 32 sines); both NULL: nothing is
+ *              rotated.  A token whose position lies outside the table leaves nothing, in no output.
+ *   neighbours 1: values 2 i and 2 i + 1 turn by angle i; 0: values i and i + 32
+ *   q_pe       [num_tokens, num_heads, 64] -> q_out, both with distances between tokens and heads in values (NULL: no queries); q_out
+ *              may be q_pe itself
+ * All vectors start on 16 bytes, MODEL1 pages on 8, others on 16.
+ */
+int smla_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_pe, int64_t k_pe_stride, void* cache, int layout,
+                   int64_t num_pages, int page_block_size, int64_t page_stride_bytes, const void* slots, int slots64,
+                   const void* positions, int positions64, const float* cos_sin, int64_t num_positions, int neighbours,
+                   const void* q_pe, int64_t q_pe_token, int64_t q_pe_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
+                   int num_tokens, int num_heads, void* stream);
+
+/*
+ * New tokens' indexer keys into the arrays that smla_mqa_logits reads, and their queries.  Values [rope_offset, rope_offset + 64) of a
+ * row of 128 are rotated as above (rope_offset 0 or 64), in fp32; then scale = max(|x|, 1e-4) / 448 and e4m3(x / scale).
+ *   k [num_tokens, 128] bf16 (rows k_stride values apart) -> ki [capacity, 128] e4m3, k_scale [capacity] fp32, at slots[t] (as above)
+ *   q [num_tokens, num_heads, 128] bf16 -> qi e4m3, w_out [num_tokens, num_heads] = weights * scale (weights NULL: the scale); q NULL: none
+ * No counterpart in the reference.
+ */
+int smla_append_index(const void* k, int64_t k_stride, void* ki, float* k_scale, int64_t capacity, const void* slots, int slots64,
+                      const void* positions, int positions64, const float* cos_sin, int64_t num_positions, int neighbours,
+                      int rope_offset, const void* q, const float* weights, void* qi, float* w_out, int num_tokens, int num_heads,
+                      void* stream);
+
+/*
+ * Attention of the newest query_len tokens of every request over all of the request's rows, found through a block table: split over the
+ * rows, joined by a second kernel.  Products of the cache's values as bf16 (exact for the packed layouts) or fp16, sums and softmax in
+ * fp32, weights rounded to the 16-bit type for their product with V.  The reference takes block_table and cache_seqlens in this place and
+ * serves index lists only (flash_mla_sm120/interface.py:39-58).
+ *   q           [batch, query_len, num_heads, 576 (512 for MODEL1)] bf16 (fp16 for SMLA_LAYOUT_F16), contiguous
+ *   block_table [batch, pages_per_request] int32, rows table_stride apart: row j of a request lies in row j % page_block_size of page
+ *               block_table[j / page_block_size]; rows in pages outside [0, num_pages) count as no entry
+ *   lengths     [batch] int32 rows of each request, the new tokens' own among them (below 0: 0; above the table: the table)
+ *   causal      1: query i sees the rows [0, length - query_len + 1 + i); 0: all
+ *   attn_sink   [num_heads] fp32 natural-log or NULL
+ *   out         [batch, query_len, num_heads, 512], lse the same without 512: base 2 with the sink in it, 0 and -1e30 where nothing is seen
+ *   num_parts   partitions that the rows of all requests are cut into (0: one per SM and 64 query rows)
+ *   scratch     smla_paged_scratch_bytes(...) bytes
+ */
+size_t smla_paged_scratch_bytes(int batch, int query_len, int num_heads, int pages_per_request, int page_block_size, int num_parts);
+int smla_paged_decode(const void* q, const void* cache, int layout, int64_t num_pages, int page_block_size, int64_t page_stride_bytes,
+                      const int32_t* block_table, int64_t table_stride, int pages_per_request, const int32_t* lengths, void* out,
+                      float* lse, int batch, int query_len, int num_heads, float sm_scale, int causal, const float* attn_sink,
+                      int num_parts, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
 
 /* Bytes of o_accum + lse_accum scratch that smla_decode_splitkv needs. */
 size_t smla_workspace_bytes(int num_tokens, int num_heads, int num_sm_parts);

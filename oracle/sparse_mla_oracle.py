@@ -571,3 +571,68 @@ def emulate_fp8_attention_dual(q: torch.Tensor, packed: torch.Tensor, indices: t
         lse[t] = row_lse
     return out.to(torch.bfloat16), lse
 
+
+
+# --------------------------------------------------------------------------- whole caches (64 bits)
+def rotate_ref(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    """x [T, ..., 64]: pair i (values 2i and 2i + 1, or i and i + 32) turned by angle i of the token's row of cos_sin [P, 32 + 32]."""
+    cs = cos_sin.double()[positions.long()].view(x.shape[0], *([1] * (x.dim() - 2)), 64)
+    c, s, x = cs[..., :32], cs[..., 32:], x.double()
+    out = torch.empty_like(x)
+    a, b = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, 32), slice(32, 64))
+    out[..., a] = x[..., a] * c - x[..., b] * s
+    out[..., b] = x[..., b] * c + x[..., a] * s
+    return out
+
+
+def cache_values(cache: torch.Tensor) -> torch.Tensor:
+    """The rows of a cache [num_blocks, block, 1, row] as 64-bit values [num_blocks, block, 576 or 512] (values that are no number stay)."""
+    if cache.dtype in (torch.bfloat16, torch.float16):
+        return cache[:, :, 0].double()
+    nb, bs, _, row = cache.shape
+    if row == ROW_BYTES:
+        p = cache[:, :, 0].contiguous()
+        scale = p[..., D_NOPE:D_NOPE + 16].contiguous().view(torch.float32).double()
+        nope = p[..., :D_NOPE].contiguous().view(torch.float8_e4m3fn).double().unflatten(-1, (NUM_TILES, QUANT_TILE)) * scale.unsqueeze(-1)
+        return torch.cat([nope.flatten(-2), p[..., D_NOPE + 16:].contiguous().view(torch.bfloat16).double()], dim=-1)
+    page = cache.reshape(nb, bs * M1_ROW_BYTES)
+    data, footer = page[:, :bs * M1_DATA_BYTES].reshape(nb, bs, M1_DATA_BYTES), page[:, bs * M1_DATA_BYTES:].reshape(nb, bs, M1_SCALE_BYTES)
+    scale = torch.exp2(footer[..., :M1_NUM_TILES].double() - 127)
+    nope = data[..., :M1_D_NOPE].contiguous().view(torch.float8_e4m3fn).double().unflatten(-1, (M1_NUM_TILES, M1_TILE)) * scale.unsqueeze(-1)
+    return torch.cat([nope.flatten(-2), data[..., M1_D_NOPE:].contiguous().view(torch.bfloat16).double()], dim=-1)
+
+
+def paged_attn_ref(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, sm_scale: float, causal: bool,
+                   attn_sink: Optional[torch.Tensor] = None):
+    """Attention of q [B, s_q, H, d] over the rows that block_table [B, pages] names, in 64 bits.  Returns (out [B, s_q, H, 512], lse base 2
+    with the sink in it, -1e30 where a query sees nothing; and, for error bounds, the same weights' sum of |v| [B, s_q, H, 512], the
+    largest sum |q_i k_i| * sm_scale over a query's rows [B, s_q, H] and the number of rows it sees [B, s_q])."""
+    B, s_q, H, _ = q.shape
+    rows = cache_values(cache)
+    page = rows.shape[1]
+    out = torch.zeros(B, s_q, H, D_V, dtype=torch.float64)
+    size = torch.zeros_like(out)
+    lse = torch.full((B, s_q, H), -1e30, dtype=torch.float64)
+    spread = torch.zeros(B, s_q, H, dtype=torch.float64)
+    seen = torch.zeros(B, s_q, dtype=torch.long)
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), block_table.shape[1] * page)
+        for i in range(s_q):
+            pos = torch.arange(max(min(n, n - s_q + 1 + i), 0) if causal else n)
+            pages = block_table[b].long()[pos // page] if len(pos) else pos
+            there = (pages >= 0) & (pages < rows.shape[0])
+            k = rows[pages[there], (pos % page)[there]]
+            sink = None if attn_sink is None else attn_sink.double()
+            if len(k) == 0:
+                if sink is not None:
+                    lse[b, i] = torch.where(sink == -math.inf, -1e30, sink / LN2)
+                continue
+            qd = q[b, i].double()
+            s = qd @ k.T * sm_scale
+            total = torch.logsumexp(s, dim=1)
+            if sink is not None:
+                total = torch.logaddexp(total, sink)
+            p = torch.exp(s - total.unsqueeze(1)) if not torch.isinf(total).any() else torch.where(torch.isinf(total).unsqueeze(1), 0.0, torch.exp(s - total.unsqueeze(1)))
+            out[b, i], size[b, i] = p @ k[:, :D_V], p @ k[:, :D_V].abs()
+            lse[b, i], spread[b, i], seen[b, i] = total / LN2, (qd.abs() @ k.abs().T).amax(dim=1) * abs(sm_scale), len(k)
+    return out, lse, size, spread, seen

@@ -9,7 +9,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 from .build import LIB_PATH, NATIVE_PATH
 
 IMPL_AUTO, IMPL_SCALAR, IMPL_TC = 0, 1, 2
-LAYOUT_V32, LAYOUT_MODEL1 = 0, 1
+LAYOUT_V32, LAYOUT_MODEL1, LAYOUT_BF16, LAYOUT_F16 = 0, 1, 2, 3
 
 _lib = None
 
@@ -53,6 +53,13 @@ _SIGS = {
     "smla_topk": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int, c_void_p]),
     "smla_topk_paged": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int, c_void_p, c_int64, c_int,
                                 c_int, c_void_p]),
+    "smla_append_kv": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p, c_int,
+                               c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "smla_append_index": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int]
+                          + [c_void_p] * 4 + [c_int, c_int, c_void_p]),
+    "smla_paged_scratch_bytes": (c_size_t, [c_int] * 6),
+    "smla_paged_decode": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                  c_int, c_int, c_int, c_float, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
     "smla_copy_batch": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "smla_cp_partition_indices": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "smla_cp_local_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),

@@ -65,6 +65,8 @@ const char* smla_status_string(int code) {
         case 33: return "attention q_staged"; case 34: return "attention q_free"; case 35: return "attention raw_empty";
         case 36: return "attention raw_full";
         case 41: return "exact attention rows free"; case 42: return "exact attention rows stored"; case 43: return "exact attention s_ready";
+        case 61: return "paged attention rows stored"; case 62: return "paged attention rows free"; case 63: return "paged attention s_ready";
+        case 64: return "paged attention p_ready"; case 65: return "paged attention pv_done"; case 66: return "paged attention q_free";
         case 51: return "attention tile k_full"; case 52: return "attention tile rope_full"; case 53: return "attention tile k_free";
         case 54: return "attention tile s_ready"; case 55: return "attention tile s_free"; case 56: return "attention tile scales";
         case 57: return "attention tile p_ready"; case 58: return "attention tile pv_done"; case 59: return "attention tile q_ready";
@@ -452,6 +454,123 @@ int smla_copy_batch(int n, void* const* dst, const void* const* src, const int64
         if (bytes[i] > 0 && (!dst[i] || !src[i])) return set_error(SMLA_E_NULL, "smla_copy_batch: null pointer argument");
     }
     return launch_copy_batch(n, dst, src, bytes, (cudaStream_t)stream);
+}
+
+static int check_layout_cache(const char* fn, const void* cache, int layout, int64_t num_pages, int page_block_size, int64_t stride, int align) {
+    static const int row[4] = {SMLA_ROW_BYTES, SMLA_M1_ROW_BYTES, 2 * SMLA_D_QK, 2 * SMLA_D_QK};
+    if (layout < SMLA_LAYOUT_V32 || layout > SMLA_LAYOUT_F16) return set_error(SMLA_E_SHAPE, "%s: unknown layout %d", fn, layout);
+    if (page_block_size < 1 || num_pages < 0 || num_pages > 0x7fffffff)
+        return set_error(SMLA_E_SHAPE, "%s: %lld pages of %d rows", fn, (long long)num_pages, page_block_size);
+    if (stride < (int64_t)page_block_size * row[layout])
+        return set_error(SMLA_E_SHAPE, "%s: page stride %lld smaller than %d rows of %d bytes", fn, (long long)stride, page_block_size, row[layout]);
+    if ((reinterpret_cast<uintptr_t>(cache) | (uintptr_t)stride) & (align - 1))
+        return set_error(SMLA_E_ALIGN, "%s: the cache and its page stride must be %d-byte aligned", fn, align);
+    return 0;
+}
+
+static int check_rotation(const char* fn, const void* positions, const float* cos_sin, int64_t num_positions) {
+    if (positions == nullptr ? cos_sin != nullptr : (cos_sin == nullptr && num_positions > 0))
+        return set_error(SMLA_E_NULL, "%s: positions and cos_sin go together", fn);
+    if (num_positions < 0) return set_error(SMLA_E_SHAPE, "%s: a table of %lld positions", fn, (long long)num_positions);
+    if (!aligned16(cos_sin)) return set_error(SMLA_E_ALIGN, "%s: cos_sin not 16-byte aligned", fn);
+    return 0;
+}
+
+int smla_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_pe, int64_t k_pe_stride, void* cache, int layout,
+                   int64_t num_pages, int page_block_size, int64_t page_stride_bytes, const void* slots, int slots64,
+                   const void* positions, int positions64, const float* cos_sin, int64_t num_positions, int neighbours,
+                   const void* q_pe, int64_t q_pe_token, int64_t q_pe_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
+                   int num_tokens, int num_heads, void* stream) {
+    const char* fn = "smla_append_kv";
+    if (num_tokens < 0 || num_heads < 0) return set_error(SMLA_E_SHAPE, "%s: tokens=%d heads=%d", fn, num_tokens, num_heads);
+    if (int e = check_layout_cache(fn, cache, layout, num_pages, page_block_size, page_stride_bytes, layout == SMLA_LAYOUT_MODEL1 ? 8 : 16)) return e;
+    if (num_tokens > 0)
+        if (int e = check_rotation(fn, positions, cos_sin, num_positions)) return e;
+    if ((q_pe == nullptr) != (q_out == nullptr)) return set_error(SMLA_E_NULL, "%s: q_pe and q_out go together", fn);
+    if (q_pe != nullptr && positions == nullptr && num_tokens > 0) return set_error(SMLA_E_NULL, "%s: queries without positions have nothing to be rotated by", fn);
+    if (num_tokens == 0) return SMLA_OK;
+    if (!kv_c || !k_pe || (!cache && num_pages > 0) || !slots) return set_error(SMLA_E_NULL, "%s: null pointer argument", fn);
+    if (!aligned16(kv_c) || !aligned16(k_pe) || !aligned16(q_pe) || !aligned16(q_out) ||
+        ((kv_c_stride | k_pe_stride | (q_pe ? q_pe_token | q_pe_head | q_out_token | q_out_head : 0)) & 7))
+        return set_error(SMLA_E_ALIGN, "%s: every vector must start on 16 bytes", fn);
+    AppendKvParams p{};
+    p.kv_c = (const uint16_t*)kv_c; p.kv_c_token = kv_c_stride; p.k_pe = (const uint16_t*)k_pe; p.k_pe_token = k_pe_stride;
+    p.cache = (uint8_t*)cache; p.page_stride = page_stride_bytes; p.page_block_size = page_block_size; p.capacity = num_pages * page_block_size;
+    p.slots = slots; p.slots64 = slots64; p.positions = positions; p.positions64 = positions64; p.cos_sin = cos_sin; p.num_positions = num_positions;
+    if (num_heads > 0) { p.q_pe = (const uint16_t*)q_pe; p.q_out = (uint16_t*)q_out; }
+    p.q_pe_token = q_pe_token; p.q_pe_head = q_pe_head; p.q_out_token = q_out_token; p.q_out_head = q_out_head;
+    p.num_tokens = num_tokens; p.num_heads = num_heads;
+    return launch_append_kv(p, layout, neighbours != 0, (cudaStream_t)stream);
+}
+
+int smla_append_index(const void* k, int64_t k_stride, void* ki, float* k_scale, int64_t capacity, const void* slots, int slots64,
+                      const void* positions, int positions64, const float* cos_sin, int64_t num_positions, int neighbours,
+                      int rope_offset, const void* q, const float* weights, void* qi, float* w_out, int num_tokens, int num_heads,
+                      void* stream) {
+    const char* fn = "smla_append_index";
+    if (num_tokens < 0 || num_heads < 0 || capacity < 0)
+        return set_error(SMLA_E_SHAPE, "%s: tokens=%d heads=%d capacity=%lld", fn, num_tokens, num_heads, (long long)capacity);
+    if (rope_offset != 0 && rope_offset != 64) return set_error(SMLA_E_SHAPE, "%s: rope_offset=%d, supported 0 and 64", fn, rope_offset);
+    if (num_tokens > 0)
+        if (int e = check_rotation(fn, positions, cos_sin, num_positions)) return e;
+    if (q != nullptr && (!qi || !w_out)) return set_error(SMLA_E_NULL, "%s: queries need qi and w_out", fn);
+    if (num_tokens == 0) return SMLA_OK;
+    if (!k || ((!ki || !k_scale) && capacity > 0) || !slots) return set_error(SMLA_E_NULL, "%s: null pointer argument", fn);
+    if (!aligned16(k) || !aligned16(ki) || !aligned16(q) || !aligned16(qi) || (k_stride & 7))
+        return set_error(SMLA_E_ALIGN, "%s: every vector must start on 16 bytes", fn);
+    AppendIndexParams p{};
+    p.k = (const uint16_t*)k; p.k_token = k_stride; p.ki = (uint8_t*)ki; p.k_scale = k_scale; p.capacity = capacity;
+    p.slots = slots; p.slots64 = slots64; p.positions = positions; p.positions64 = positions64; p.cos_sin = cos_sin; p.num_positions = num_positions;
+    p.rope_offset = rope_offset; p.num_tokens = num_tokens; p.num_heads = num_heads;
+    if (num_heads > 0) { p.q = (const uint16_t*)q; p.weights = weights; p.qi = (uint8_t*)qi; p.w_out = w_out; }
+    return launch_append_index(p, neighbours != 0, (cudaStream_t)stream);
+}
+
+static int paged_shape(const char* fn, int batch, int query_len, int num_heads, int pages_per_request, int page_block_size, int num_parts) {
+    if (batch < 0 || query_len < 0 || num_heads < 1 || num_heads > 128 || pages_per_request < 0 || page_block_size < 1 || num_parts < 0)
+        return set_error(SMLA_E_SHAPE, "%s: batch=%d query_len=%d num_heads=%d (supported 1..128) pages=%d of %d num_parts=%d", fn, batch, query_len, num_heads,
+                         pages_per_request, page_block_size, num_parts);
+    if ((int64_t)query_len * num_heads > 64 * 65535 || num_parts > 65536)
+        return set_error(SMLA_E_SHAPE, "%s: %d queries of %d heads, %d partitions", fn, query_len, num_heads, num_parts);
+    return 0;
+}
+
+static size_t paged_lse_at(int parts, size_t rows) { return parts > 1 ? 2 * (size_t)parts * rows * SMLA_D_V * sizeof(float) : 0; }
+static size_t paged_spans_at(int parts, size_t rows) {
+    return paged_lse_at(parts, rows) + (parts > 1 ? (2 * (size_t)parts * rows * sizeof(float) + 15) / 16 * 16 : 0);
+}
+
+size_t smla_paged_scratch_bytes(int batch, int query_len, int num_heads, int pages_per_request, int page_block_size, int num_parts) {
+    if (paged_shape("smla_paged_scratch_bytes", batch, query_len, num_heads, pages_per_request, page_block_size, num_parts)) return 0;
+    const int parts = paged_parts(batch, query_len * num_heads, pages_per_request, page_block_size, num_parts);
+    return parts < 1 ? 0 : paged_spans_at(parts, (size_t)query_len * num_heads) + (size_t)batch * sizeof(int2);
+}
+
+int smla_paged_decode(const void* q, const void* cache, int layout, int64_t num_pages, int page_block_size, int64_t page_stride_bytes,
+                      const int32_t* block_table, int64_t table_stride, int pages_per_request, const int32_t* lengths, void* out,
+                      float* lse, int batch, int query_len, int num_heads, float sm_scale, int causal, const float* attn_sink,
+                      int num_parts, void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
+    const char* fn = "smla_paged_decode";
+    if (int e = paged_shape(fn, batch, query_len, num_heads, pages_per_request, page_block_size, num_parts)) return e;
+    if (int e = check_layout_cache(fn, cache, layout, num_pages, page_block_size, page_stride_bytes, 16)) return e;
+    if (table_stride < 0) return set_error(SMLA_E_SHAPE, "%s: table stride %lld", fn, (long long)table_stride);
+    if (batch == 0 || query_len == 0) return SMLA_OK;
+    if (!q || (!cache && num_pages > 0) || (!block_table && pages_per_request > 0) || !lengths || !out || !lse || !scratch) return set_error(SMLA_E_NULL, "%s: null pointer argument", fn);
+    if (!aligned16(q) || !aligned16(out) || !aligned16(scratch)) return set_error(SMLA_E_ALIGN, "%s: q, out and scratch must be 16-byte aligned", fn);
+    PagedParams p{};
+    p.rows = query_len * num_heads;
+    p.num_parts = paged_parts(batch, p.rows, pages_per_request, page_block_size, num_parts);
+    if (p.num_parts < 1) return SMLA_E_DEVICE;
+    const size_t need = paged_spans_at(p.num_parts, p.rows) + (size_t)batch * sizeof(int2);
+    if (scratch_bytes < need) return set_error(SMLA_E_WORKSPACE, "%s: %zu bytes of scratch, %zu needed", fn, scratch_bytes, need);
+    p.q = (const uint8_t*)q; p.cache = (const uint8_t*)cache; p.page_stride = page_stride_bytes; p.num_pages = (int)num_pages;
+    p.page_block_size = page_block_size; p.table = block_table; p.table_stride = table_stride; p.pages_per_request = pages_per_request;
+    p.lengths = lengths; p.attn_sink = attn_sink; p.out = out; p.lse = lse;
+    p.o_part = (float*)scratch;
+    p.lse_part = (float*)((char*)scratch + paged_lse_at(p.num_parts, p.rows));
+    p.spans = (int2*)((char*)scratch + paged_spans_at(p.num_parts, p.rows));
+    p.status = status; p.batch = batch; p.query_len = query_len; p.num_heads = num_heads; p.causal = causal != 0; p.sm_scale = sm_scale;
+    return launch_attn_paged(p, layout, (cudaStream_t)stream);
 }
 
 int smla_cp_partition_indices(const int32_t* indices, int32_t* local_indices, int32_t* local_length,

@@ -154,6 +154,44 @@ inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 bl
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// New tokens' rows and queries (append.cu).  Distances between tokens and heads in values; the launchers set `parts`.
+struct AppendKvParams {
+    const uint16_t* kv_c; int64_t kv_c_token;
+    const uint16_t* k_pe; int64_t k_pe_token;
+    uint8_t* cache; int64_t page_stride, capacity; int page_block_size;
+    const void* slots; int slots64;
+    const void* positions; int positions64;
+    const float* cos_sin; int64_t num_positions;
+    const uint16_t* q_pe; int64_t q_pe_token, q_pe_head;
+    uint16_t* q_out; int64_t q_out_token, q_out_head;
+    int num_tokens, num_heads, parts;
+};
+struct AppendIndexParams {
+    const uint16_t* k; int64_t k_token;
+    uint8_t* ki; float* k_scale; int64_t capacity;
+    const void* slots; int slots64;
+    const void* positions; int positions64;
+    const float* cos_sin; int64_t num_positions; int rope_offset;
+    const uint16_t* q; const float* weights; uint8_t* qi; float* w_out;
+    int num_tokens, num_heads, parts;
+};
+
+// Attention over the rows of a block table (paged.cu).
+struct PagedParams {
+    const uint8_t* q;            // [batch, rows, 576 or 512] 16-bit; rows = query_len * num_heads
+    const uint8_t* cache; int64_t page_stride; int num_pages, page_block_size;
+    const int32_t* table; int64_t table_stride; int pages_per_request;
+    const int32_t* lengths;
+    const float* attn_sink;      // [num_heads] or null
+    void* out; float* lse;
+    float* o_part;               // [2 num_parts][rows][512]: record 2 c + 1 of partition c for the request that begins in it, 2 c for one before
+    float* lse_part;             // [2 num_parts][rows]
+    int2* spans;                 // [batch]: first and last partition of a request
+    int32_t* status;
+    int batch, query_len, num_heads, rows, num_parts, causal;
+    float sm_scale;
+};
+
 // Host-side error plumbing (api.cu).
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
@@ -187,6 +225,10 @@ bool attn_duo_takes(const AttnParams& p);    // the same caches, the calls that 
 int launch_attn_duo(const AttnParams& p, cudaStream_t stream);
 int launch_attn_exact(const AttnParams& p, cudaStream_t stream);   // MODEL1 layout, caches aligned as for the pair kernel
 bool attn_pair_takes(const AttnParams& p);   // alignment of the caches that the tensor-core kernel's bulk copies need
+int launch_append_kv(AppendKvParams p, int layout, bool pairs, cudaStream_t stream);
+int launch_append_index(AppendIndexParams p, bool pairs, cudaStream_t stream);
+int paged_parts(int batch, int rows, int pages_per_request, int page_block_size, int num_parts);   // partitions of a call, 0: an error is set
+int launch_attn_paged(const PagedParams& p, int layout, cudaStream_t stream);
 int launch_pack_kv(const __nv_bfloat16* kv, uint8_t* packed, int64_t num_rows, cudaStream_t stream);
 int launch_mqa_logits_scalar(const uint8_t* q, const uint8_t* k, const float* k_scale, const float* weights,
                              const int32_t* ks, const int32_t* ke, float* logits, int s_q, int num_heads,

@@ -17,6 +17,7 @@
 
 #include <cstdarg>
 #include <map>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -38,6 +39,10 @@ struct Api {
     decltype(&smla_topk) topk;
     decltype(&smla_topk_paged) topk_paged;
     decltype(&smla_copy_batch) copy_batch;
+    decltype(&smla_append_kv) append_kv;
+    decltype(&smla_append_index) append_index;
+    decltype(&smla_paged_scratch_bytes) paged_scratch_bytes;
+    decltype(&smla_paged_decode) paged_decode;
 } api;
 PyObject* g_runtime = nullptr;      // module _runtime: split policy, status buffer, default numerics of MODEL1
 PyObject* g_error = nullptr;        // SmlaError
@@ -466,6 +471,198 @@ PyObject* copy_into(const Args& x) {
     Py_RETURN_NONE;
 }
 
+// Layout, pages and page geometry of a cache that rows are appended to or a block table points into: the byte layouts, or rows of 576
+// bf16 or fp16 values [num_blocks, block, 1, 576].
+struct Pages {
+    int layout;
+    int64_t pages, block, stride;
+};
+Pages pages_of(const at::Tensor& kv) {
+    Pages g{};
+    const auto t = kv.scalar_type();
+    if (t == at::kBFloat16 || t == at::kHalf) {
+        if (kv.dim() != 4 || kv.size(2) != 1 || kv.size(3) != SMLA_D_QK || kv.stride(3) != 1 || (kv.size(1) > 1 && kv.stride(1) != SMLA_D_QK))
+            fail(PyExc_ValueError, "a cache of 16-bit rows must be [num_blocks, block, 1, 576] with contiguous rows");
+        g.layout = t == at::kHalf ? SMLA_LAYOUT_F16 : SMLA_LAYOUT_BF16;
+        g.pages = kv.size(0); g.block = kv.size(1); g.stride = kv.stride(0) * 2;
+    } else {
+        const Cache c = geometry(kv);
+        g.layout = c.layout; g.block = c.block; g.stride = c.stride;
+        g.pages = kv.dim() == 4 ? kv.size(0) : (kv.size(0) > 0 ? 1 : 0);
+    }
+    if (g.block < 1 || g.block > 0x7fffffff) fail(PyExc_ValueError, "kv_cache has pages of %lld rows", (long long)g.block);
+    const int64_t row = g.layout == SMLA_LAYOUT_V32 ? SMLA_ROW_BYTES : g.layout == SMLA_LAYOUT_MODEL1 ? SMLA_M1_ROW_BYTES : 2 * SMLA_D_QK;
+    if (g.pages <= 1) g.stride = (g.block * row + 15) / 16 * 16;      // a single page has no distance to the next
+    return g;
+}
+
+// Which row of the cache each token goes to, and its row in the table of cosines and sines.
+struct Places {
+    at::Tensor slots, positions, cos_sin;
+    int64_t tokens = 0;
+    static void index(const at::Tensor& t, const char* name, int64_t n) {
+        if ((t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
+            fail(PyExc_ValueError, "%s must be contiguous int32 or int64 [%lld]", name, (long long)n);
+    }
+    void check(int64_t n) {
+        tokens = n;
+        if (n > 0x7fffffff) fail(PyExc_ValueError, "%lld tokens", (long long)n);
+        index(slots, "slot_mapping", n);
+        if (positions.defined() != cos_sin.defined()) fail(PyExc_ValueError, "positions and cos_sin go together");
+        if (!positions.defined()) return;
+        index(positions, "positions", n);
+        if (cos_sin.scalar_type() != at::kFloat || cos_sin.dim() != 2 || cos_sin.size(1) != 64 || !cos_sin.is_contiguous())
+            fail(PyExc_ValueError, "cos_sin must be contiguous float32 [positions, 64]: 32 cosines, 32 sines");
+    }
+    int slots64() const { return slots.scalar_type() == at::kLong; }
+    int positions64() const { return positions.defined() && positions.scalar_type() == at::kLong; }
+    int64_t rows() const { return cos_sin.defined() ? cos_sin.size(0) : 0; }
+};
+
+int64_t distance(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }      // between neighbours of dimension d, if it has any
+
+void require_type(const at::Tensor& t, const char* name, at::ScalarType type, std::initializer_list<int64_t> shape) {
+    bool ok = t.scalar_type() == type && t.dim() == (int64_t)shape.size() && t.numel() >= 0;
+    std::string want;
+    int64_t d = 0;
+    for (const int64_t n : shape) {
+        ok = ok && t.size(d) == n;
+        want += (d++ ? ", " : "") + std::to_string(n);
+    }
+    if (!ok) fail(PyExc_ValueError, "%s must be %s [%s]", name, c10::toString(type), want.c_str());
+}
+
+// (kv_c, k_pe, kv_cache, slot_mapping, positions, cos_sin, interleaved, q_pe, q_out) -> q_out or None
+PyObject* append_kv(const Args& x) {
+    const at::Tensor kv_c = x.needed(0), k_pe = x.needed(1), kv = x.needed(2), q_pe = x.tensor(7);
+    at::Tensor q_out = x.tensor(8);
+    Places at;
+    at.slots = x.needed(3); at.positions = x.tensor(4); at.cos_sin = x.tensor(5);
+    const Pages g = pages_of(kv);
+    const auto type = g.layout == SMLA_LAYOUT_F16 ? at::kHalf : at::kBFloat16;
+    if (kv_c.dim() != 2) fail(PyExc_ValueError, "kv_c must be [num_tokens, %d]", g.layout == SMLA_LAYOUT_MODEL1 ? 448 : 512);
+    const int64_t n = kv_c.size(0);
+    require_type(kv_c, "kv_c", type, {n, g.layout == SMLA_LAYOUT_MODEL1 ? 448 : 512});
+    require_type(k_pe, "k_pe", type, {n, 64});
+    if (n > 0 && (kv_c.stride(1) != 1 || k_pe.stride(1) != 1)) fail(PyExc_ValueError, "the rows of kv_c and k_pe must be contiguous");
+    at.check(n);
+    int64_t heads = 0;
+    if (q_pe.defined()) {
+        if (!at.positions.defined()) fail(PyExc_ValueError, "q_pe needs positions and cos_sin");
+        if (q_pe.dim() != 3) fail(PyExc_ValueError, "q_pe must be [num_tokens, num_heads, 64]");
+        heads = q_pe.size(1);
+        require_type(q_pe, "q_pe", type, {n, heads, 64});
+        if (q_out.defined()) require_type(q_out, "q_out", type, {n, heads, 64});
+        if (q_pe.numel() > 0 && (q_pe.stride(2) != 1 || (q_out.defined() && q_out.stride(2) != 1))) fail(PyExc_ValueError, "the vectors of q_pe and q_out must be contiguous");
+    } else if (q_out.defined()) {
+        fail(PyExc_ValueError, "q_out without q_pe");
+    }
+    require_cuda({&kv_c, &k_pe, &kv, &at.slots, &at.positions, &at.cos_sin, &q_pe, &q_out});
+    require_one_device(kv, {&kv_c, &k_pe, &at.slots, &at.positions, &at.cos_sin, &q_pe, &q_out});
+    const c10::cuda::CUDAGuard on(kv.device());
+    if (q_pe.defined() && !q_out.defined()) q_out = at::empty({n, heads, 64}, q_pe.options());
+    const int pairs = (int)x.integer(6);
+    launch([&] {
+        const bool q = q_pe.defined() && q_pe.numel() > 0;
+        return api.append_kv(ptr(kv_c), distance(kv_c, 0), ptr(k_pe), distance(k_pe, 0), ptr(kv), g.layout, g.pages, (int)g.block, g.stride,
+                             ptr(at.slots), at.slots64(), ptr(at.positions), at.positions64(), ptr_as<float>(at.cos_sin), at.rows(), pairs,
+                             q ? ptr(q_pe) : nullptr, q ? distance(q_pe, 0) : 0, q ? distance(q_pe, 1) : 0, q ? ptr(q_out) : nullptr,
+                             q ? distance(q_out, 0) : 0, q ? distance(q_out, 1) : 0, (int)n, (int)heads, stream_of(kv));
+    });
+    if (!q_out.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(q_out);
+}
+
+// (k, ki, k_scale, slot_mapping, positions, cos_sin, interleaved, rope_offset, q, weights) -> (qi, weights) or None
+PyObject* append_index(const Args& x) {
+    const at::Tensor k = x.needed(0), ki = x.needed(1), k_scale = x.needed(2), q = x.tensor(8), w = x.tensor(9);
+    Places at;
+    at.slots = x.needed(3); at.positions = x.tensor(4); at.cos_sin = x.tensor(5);
+    if (k.dim() != 2 || ki.dim() != 2) fail(PyExc_ValueError, "k must be [num_tokens, 128] and ki [s_k, 128]");
+    const int64_t n = k.size(0);
+    require_type(k, "k", at::kBFloat16, {n, 128});
+    require_type(ki, "ki", at::kFloat8_e4m3fn, {ki.size(0), 128});
+    require_type(k_scale, "k_scale", at::kFloat, {ki.size(0)});
+    if (!ki.is_contiguous() || !k_scale.is_contiguous() || (n > 0 && k.stride(1) != 1)) fail(PyExc_ValueError, "ki, k_scale and the rows of k must be contiguous");
+    at.check(n);
+    int64_t heads = 0;
+    if (q.defined()) {
+        if (q.dim() != 3) fail(PyExc_ValueError, "q must be [num_tokens, num_heads, 128]");
+        heads = q.size(1);
+        require_type(q, "q", at::kBFloat16, {n, heads, 128});
+        if (w.defined()) require_type(w, "weights", at::kFloat, {n, heads});
+        if (!q.is_contiguous() || (w.defined() && !w.is_contiguous())) fail(PyExc_ValueError, "q and weights must be contiguous");
+    } else if (w.defined()) {
+        fail(PyExc_ValueError, "weights without q");
+    }
+    require_cuda({&k, &ki, &k_scale, &at.slots, &at.positions, &at.cos_sin, &q, &w});
+    require_one_device(k, {&ki, &k_scale, &at.slots, &at.positions, &at.cos_sin, &q, &w});
+    const c10::cuda::CUDAGuard on(k.device());
+    at::Tensor qi, w_out;
+    if (q.defined()) {
+        qi = at::empty({n, heads, 128}, q.options().dtype(at::kFloat8_e4m3fn));
+        w_out = at::empty({n, heads}, q.options().dtype(at::kFloat));
+    }
+    const int pairs = (int)x.integer(6), offset = (int)x.integer(7);
+    launch([&] {
+        const bool some = q.defined() && q.numel() > 0;
+        return api.append_index(ptr(k), distance(k, 0), ptr(ki), ptr_as<float>(k_scale), ki.size(0), ptr(at.slots), at.slots64(), ptr(at.positions),
+                                at.positions64(), ptr_as<float>(at.cos_sin), at.rows(), pairs, offset, some ? ptr(q) : nullptr, ptr_as<float>(w),
+                                some ? ptr(qi) : nullptr, some ? ptr_as<float>(w_out) : nullptr, (int)n, (int)heads, stream_of(k));
+    });
+    if (!q.defined()) Py_RETURN_NONE;
+    return wrap2(qi, w_out);
+}
+
+// (q, kv_cache, block_table, cache_seqlens, sm_scale, d_v, causal, attn_sink, out, num_sm_parts) -> (out, lse)
+PyObject* paged_decode(const Args& x) {
+    const at::Tensor q = x.needed(0), kv = x.needed(1), table = x.needed(2), lens = x.needed(3), sink = x.tensor(7);
+    at::Tensor out = x.tensor(8);
+    if (kv.dim() != 4) fail(PyExc_ValueError, "kv_cache must be [num_blocks, block, 1, 656 | 584 bytes | 576 bf16 or fp16 values]");
+    const Pages g = pages_of(kv);
+    const auto type = g.layout == SMLA_LAYOUT_F16 ? at::kHalf : at::kBFloat16;
+    const int64_t d = g.layout == SMLA_LAYOUT_MODEL1 ? SMLA_M1_D_QK : SMLA_D_QK;
+    if ((q.dim() != 3 && q.dim() != 4) || q.scalar_type() != type || q.size(-1) != d)
+        fail(PyExc_ValueError, "q must be %s [batch, num_heads, %lld] or [batch, s_q, num_heads, %lld] for this cache", c10::toString(type), (long long)d, (long long)d);
+    if (!q.is_contiguous()) fail(PyExc_ValueError, "q must be contiguous");
+    if (x.integer(5) != SMLA_D_V) fail(PyExc_ValueError, "d_v must be 512, got %lld", (long long)x.integer(5));
+    const int64_t n = q.size(0), s_q = q.dim() == 4 ? q.size(1) : 1, heads = q.size(-2);
+    if (n > 0x7fffffff || s_q > 0x7fffffff || heads > 0x7fffffff) fail(PyExc_ValueError, "q is too large");
+    if (table.dim() != 2 || table.scalar_type() != at::kInt || table.size(0) != n || (table.size(1) > 1 && table.stride(1) != 1) || table.size(1) > 0x7fffffff)
+        fail(PyExc_ValueError, "block_table must be int32 [%lld, pages] with contiguous rows", (long long)n);
+    if (lens.dim() != 1 || lens.scalar_type() != at::kInt || lens.size(0) != n || !lens.is_contiguous())
+        fail(PyExc_ValueError, "cache_seqlens must be contiguous int32 [%lld]", (long long)n);
+    if (sink.defined() && (sink.scalar_type() != at::kFloat || sink.numel() != heads || !sink.is_contiguous()))
+        fail(PyExc_ValueError, "attn_sink must be contiguous float32 [%lld]", (long long)heads);
+    auto shape = q.sizes().vec();
+    shape.back() = SMLA_D_V;
+    if (out.defined() && (out.sizes() != at::IntArrayRef(shape) || out.scalar_type() != type || !out.is_contiguous()))
+        fail(PyExc_ValueError, "out must be contiguous, of q's type and shape with 512 values in the last dimension");
+    require_cuda({&q, &kv, &table, &lens, &sink, &out});
+    require_one_device(q, {&kv, &table, &lens, &sink, &out});
+    const c10::cuda::CUDAGuard on(q.device());
+    if (!out.defined()) out = at::empty(shape, q.options());
+    shape.pop_back();
+    const at::Tensor lse = at::empty(shape, q.options().dtype(at::kFloat));
+    const int64_t parts = x.none(9) ? 0 : x.integer(9);
+    if (!x.none(9) && (parts < 1 || parts > 65536)) fail(PyExc_ValueError, "num_sm_parts must be 1 to 65536, got %lld", (long long)parts);
+    if (q.numel() == 0 && (n == 0 || s_q == 0)) return wrap2(out, lse);
+    const int pages = (int)table.size(1);
+    const size_t bytes = api.paged_scratch_bytes((int)n, (int)s_q, (int)heads, pages, (int)g.block, (int)parts);
+    if (bytes == 0) fail(PyExc_ValueError, "%s", api.last_error());
+    // scratch of this call alone, as in decode()
+    const at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    const float scale = (float)x.real(4);
+    const int causal = (int)x.integer(6);
+    int32_t* status = status_of(q);
+    launch([&] {
+        return api.paged_decode(ptr(q), ptr(kv), g.layout, g.pages, (int)g.block, g.stride, ptr_as<int32_t>(table), n > 1 ? table.stride(0) : pages, pages,
+                                ptr_as<int32_t>(lens), ptr(out), ptr_as<float>(lse), (int)n, (int)s_q, (int)heads, scale, causal, ptr_as<float>(sink),
+                                (int)parts, ptr(ws), bytes, status, stream_of(q));
+    });
+    return wrap2(out, lse);
+}
+
 // (handle of the loaded library, module _runtime, SmlaError)
 PyObject* init(const Args& x) {
     void* lib = reinterpret_cast<void*>((uintptr_t)x.integer(0));
@@ -478,6 +675,8 @@ PyObject* init(const Args& x) {
     get(api.prefill_ext, "smla_prefill_ext"); get(api.combine, "smla_combine"); get(api.pack_kv, "smla_pack_kv");
     get(api.mqa_logits, "smla_mqa_logits"); get(api.topk, "smla_topk");
     get(api.topk_paged, "smla_topk_paged"); get(api.copy_batch, "smla_copy_batch");
+    get(api.append_kv, "smla_append_kv"); get(api.append_index, "smla_append_index");
+    get(api.paged_scratch_bytes, "smla_paged_scratch_bytes"); get(api.paged_decode, "smla_paged_decode");
     g_runtime = x.a[1]; Py_INCREF(g_runtime);
     g_error = x.a[2]; Py_INCREF(g_error);
     Py_RETURN_NONE;
@@ -500,7 +699,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     SMLA_FN("init", init, 3, false), SMLA_FN("decode", decode, 14), SMLA_FN("prefill", prefill, 12),
     SMLA_FN("mqa_logits", mqa_logits, 8), SMLA_FN("topk", topk, 6), SMLA_FN("pack_kv", pack_kv, 1),
-    SMLA_FN("copy_into", copy_into, 2),
+    SMLA_FN("copy_into", copy_into, 2), SMLA_FN("append_kv", append_kv, 9), SMLA_FN("append_index", append_index, 10),
+    SMLA_FN("paged_decode", paged_decode, 10),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_smla_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

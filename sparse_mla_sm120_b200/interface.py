@@ -13,8 +13,9 @@ layer with the same metadata object) can switch over:
   the later ones.  Here the object also keeps the split-KV scratch, and when every request gets
   its own partition there is nothing to schedule: the attention kernel runs alone.
 
-Only sparse attention over an FP8 cache is served (as in the reference).  Both cache layouts and the
-second ("extra") cache are taken; see flash_ops for which kernel serves which.
+Sparse attention is served over an FP8 cache (as in the reference), in both cache layouts and with the
+second ("extra") cache; see flash_ops for which kernel serves which.  Calls without ``indices`` attend to all rows
+(paged.paged_mla_decode_fwd).
 """
 from __future__ import annotations
 
@@ -28,6 +29,7 @@ from ._lib import IMPL_AUTO, IMPL_SCALAR, LAYOUT_V32, check
 from ._runtime import (BLOCK_N, kv_geometry, one_array, ptr, require_cuda, resolve_impl, split_plan, status_buffer, stream_ptr,
                        tc_aligned)
 from .flash_ops import _check_q, _Extra, _layout, sparse_mla_prefill_fwd
+from .paged import paged_mla_decode_fwd
 
 
 @dataclasses.dataclass
@@ -85,17 +87,20 @@ def flash_mla_with_kvcache(
     out: Optional[torch.Tensor] = None,
     impl: int = IMPL_AUTO,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Sparse decode over a paged FP8 cache (interface.py:39-171).  ``block_table`` and
-    ``cache_seqlens`` are accepted and unused, as in the reference: ``indices`` are physical rows."""
+    """Sparse decode over a paged FP8 cache (interface.py:39-171).  With ``indices``, ``block_table`` and
+    ``cache_seqlens`` are accepted and unused, as in the reference: ``indices`` are physical rows.  Without, the
+    ``s_q`` queries of request b see all of its ``cache_seqlens[b]`` rows (``causal``: up to their own), found through
+    ``block_table``, in either FP8 layout or, where ``is_fp8_kvcache`` is false, in rows of 576 bf16 or fp16 values."""
     meta = tile_scheduler_metadata
     if not isinstance(meta, FlashMLASchedMeta):
         raise TypeError("tile_scheduler_metadata must come from get_mla_metadata()")
     if num_splits is not None:
         raise ValueError("num_splits must be None (the metadata object carries it)")
     if indices is None:
-        raise ValueError("only sparse attention is served: indices is required")
+        return _attend_to_all(q, k_cache, block_table, cache_seqlens, head_dim_v, meta, softmax_scale, causal, is_fp8_kvcache,
+                              attn_sink, (extra_k_cache, extra_indices_in_kvcache, topk_length, extra_topk_length), out)
     if not is_fp8_kvcache:
-        raise ValueError("an FP8 KV cache is required")
+        raise ValueError("sparse attention needs an FP8 KV cache")
     if head_dim_v != 512:
         raise ValueError(f"head_dim_v must be 512, got {head_dim_v}")
     if softmax_scale is None:
@@ -182,6 +187,29 @@ def flash_mla_with_kvcache(
     output = output.reshape(batch, s_q, num_heads, head_dim_v)
     lse = out_lse.reshape(batch, s_q, num_heads).permute(0, 2, 1).contiguous()
     return output, lse
+
+
+def _attend_to_all(q, k_cache, block_table, cache_seqlens, head_dim_v, meta, softmax_scale, causal, is_fp8_kvcache, attn_sink, sparse_only, out):
+    """The calls without ``indices``."""
+    if block_table is None or cache_seqlens is None:
+        raise ValueError("either indices, or block_table and cache_seqlens")
+    if any(t is not None for t in sparse_only):
+        raise ValueError("a second cache and topk_length go with indices")
+    if is_fp8_kvcache != (k_cache.dtype not in (torch.bfloat16, torch.float16)):
+        raise ValueError(f"is_fp8_kvcache={is_fp8_kvcache} does not go with a cache of {k_cache.dtype}")
+    if q.dim() not in (3, 4) or k_cache.dim() != 4:
+        raise ValueError("q must be [b, s_q, h_q, d] or [b, h_q, d] and k_cache [num_blocks, block, 1, row]")
+    cfg = FlashMLASchedMeta.Config(b=q.shape[0], s_q=q.shape[1] if q.dim() == 4 else 1, h_q=q.shape[-2], page_block_size=k_cache.shape[1],
+                                   h_k=k_cache.shape[2], causal=causal, is_fp8_kvcache=is_fp8_kvcache, topk=None,
+                                   extra_page_block_size=None, extra_topk=None)
+    if meta.have_initialized and meta.config != cfg:
+        raise ValueError(f"the metadata object was initialised for {meta.config}, this call has {cfg}")
+    shape = (cfg.b, cfg.s_q, cfg.h_q)
+    output, lse = paged_mla_decode_fwd(q.contiguous().view(*shape, q.shape[-1]), k_cache, block_table, cache_seqlens,
+                                       q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale, head_dim_v, causal, attn_sink,
+                                       None if out is None else out.view(*shape, head_dim_v))
+    meta.have_initialized, meta.config = True, cfg
+    return output, lse.permute(0, 2, 1).contiguous()
 
 
 def flash_mla_sparse_fwd(

@@ -67,6 +67,7 @@ const char* smla_status_string(int code) {
         case 41: return "exact attention rows free"; case 42: return "exact attention rows stored"; case 43: return "exact attention s_ready";
         case 61: return "paged attention rows stored"; case 62: return "paged attention rows free"; case 63: return "paged attention s_ready";
         case 64: return "paged attention p_ready"; case 65: return "paged attention pv_done"; case 66: return "paged attention q_free";
+        case 67: return "paged attention s_free";
         case 51: return "attention tile k_full"; case 52: return "attention tile rope_full"; case 53: return "attention tile k_free";
         case 54: return "attention tile s_ready"; case 55: return "attention tile s_free"; case 56: return "attention tile scales";
         case 57: return "attention tile p_ready"; case 58: return "attention tile pv_done"; case 59: return "attention tile q_ready";
@@ -562,6 +563,7 @@ int smla_paged_decode(const void* q, const void* cache, int layout, int64_t num_
     p.num_parts = paged_parts(batch, p.rows, pages_per_request, page_block_size, num_parts);
     if (p.num_parts < 1) return SMLA_E_DEVICE;
     const size_t need = paged_spans_at(p.num_parts, p.rows) + (size_t)batch * sizeof(int2);
+    if ((int64_t)batch * p.rows > 0x7fffffff) return set_error(SMLA_E_SHAPE, "%s: batch=%d of %d query rows", fn, batch, p.rows);
     if (scratch_bytes < need) return set_error(SMLA_E_WORKSPACE, "%s: %zu bytes of scratch, %zu needed", fn, scratch_bytes, need);
     p.q = (const uint8_t*)q; p.cache = (const uint8_t*)cache; p.page_stride = page_stride_bytes; p.num_pages = (int)num_pages;
     p.page_block_size = page_block_size; p.table = block_table; p.table_stride = table_stride; p.pages_per_request = pages_per_request;

@@ -189,6 +189,7 @@ struct PagedParams {
     int2* spans;                 // [batch]: first and last partition of a request
     int32_t* status;
     int batch, query_len, num_heads, rows, num_parts, causal;
+    int copy_rows;               // rows of one TMA copy (set by the launcher)
     float sm_scale;
 };
 
@@ -228,7 +229,7 @@ bool attn_pair_takes(const AttnParams& p);   // alignment of the caches that the
 int launch_append_kv(AppendKvParams p, int layout, bool pairs, cudaStream_t stream);
 int launch_append_index(AppendIndexParams p, bool pairs, cudaStream_t stream);
 int paged_parts(int batch, int rows, int pages_per_request, int page_block_size, int num_parts);   // partitions of a call, 0: an error is set
-int launch_attn_paged(const PagedParams& p, int layout, cudaStream_t stream);
+int launch_attn_paged(PagedParams p, int layout, cudaStream_t stream);
 int launch_pack_kv(const __nv_bfloat16* kv, uint8_t* packed, int64_t num_rows, cudaStream_t stream);
 int launch_mqa_logits_scalar(const uint8_t* q, const uint8_t* k, const float* k_scale, const float* weights,
                              const int32_t* ks, const int32_t* ke, float* logits, int s_q, int num_heads,

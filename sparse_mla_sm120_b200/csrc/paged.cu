@@ -13,11 +13,13 @@
 //   S [64 x 64] = Q . K^T: A = Q, B = 64 cache rows, both K-major in chunks of 64 dims, 128B swizzle;
 //   O^T [4 x 128 dims x rows] += V^T . P^T: A = the same rows read MN-major, B = the weights, a line of 64 rows' weights per query row.
 // O has to be transposed: 64 x 512 fp32 fill half of tensor memory that way, all of it the other way.
-// Warps: 0-3 softmax, epilogue; 4-7 and 8-11 bring the rows of even and odd blocks into two stages of 72 KB, 16-bit rows by
-// cp.async, packed rows through registers (e4m3 x its scale is exact in bf16); 12 issues the MMAs: scores of a block as soon as its
-// rows are there, P.V of the one before as soon as its weights are.
+// Warps: 0-7 softmax and epilogue (16 query rows by half of the block's rows each); one that issues the score MMAs and one for P.V; and
+// who brings the rows into two stages of 72 KB: one warp by TMA (16-bit rows), or eight through registers (packed rows: e4m3 x its scale
+// is exact in bf16; four for even blocks, four for odd ones).  A stage is filled and freed in four groups of 128 dims, so that scores
+// begin when a quarter of the rows is there, and the next rows come when P.V is through with a quarter.
 // Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
 #include "attn_common.cuh"
+#include "rows_map.cuh"
 #include "sm100_ptx.cuh"
 
 namespace smla {
@@ -30,11 +32,17 @@ using namespace attn;
 constexpr int PG_ROWS = 64;                       // query rows of a CTA
 constexpr int PG_START = 2;                       // blocks' worth of time that a request takes before its first row
 constexpr int PG_LEAST = 2;                       // blocks of rows that a partition should be worth
-constexpr int PG_SM_WARPS = 4, PG_LD_WARPS = 8, PG_MMA_WARP = PG_SM_WARPS + PG_LD_WARPS;
-constexpr int PG_THREADS = (PG_MMA_WARP + 1) * 32;
+constexpr int PG_SM_WARPS = 8, PG_SM_THREADS = PG_SM_WARPS * 32;
+__host__ __device__ constexpr bool packed_rows(int layout) { return layout == SMLA_LAYOUT_V32 || layout == SMLA_LAYOUT_MODEL1; }
+__host__ __device__ constexpr int load_warps(int layout) { return packed_rows(layout) ? 8 : 4; }
+__host__ __device__ constexpr int paged_threads(int layout) { return packed_rows(layout) ? 640 : 448; }       // (packed: whole groups of four warps)
 // The running maximum of a row lags by at most 2^PG_TAU: weights are floating point, so that costs no precision (fp16 weights reach
 // 2^8 and fall to zero 2^-24 below a maximum that does not lag), and the accumulator is rescaled a few times per request.
 constexpr float PG_TAU = 8.0f;
+
+// registers of the packed layouts' instances, which the loading warps take from the others
+constexpr int PG_REGS_LAUNCH = 96, PG_REGS_SOFTMAX = 88, PG_REGS_LOAD = 120, PG_REGS_MMA = 48;
+static_assert(PG_SM_WARPS * 32 * PG_REGS_SOFTMAX + 8 * 32 * PG_REGS_LOAD + 4 * 32 * PG_REGS_MMA <= 640 * PG_REGS_LAUNCH, "register budgets exceed what the CTA owns");
 
 constexpr uint32_t G_CHUNK = 64 * 128;            // 64 dims of 64 rows
 constexpr uint32_t G_STAGE = 9 * G_CHUNK;
@@ -44,9 +52,11 @@ constexpr uint32_t GP_OFF = GK_OFF + 2 * G_STAGE;             // weights [64 que
 constexpr uint32_t GV_OFF = GP_OFF + G_CHUNK;                 // validity: a bit per row, [2 stages] 64 bits
 constexpr uint32_t GN_OFF = GV_OFF + 16;                      // rows that some query must not see and whose values are no numbers
 constexpr uint32_t GA_OFF = GN_OFF + 16;                      // [64] fp32: rescale factors, then 1 / denominator
-constexpr uint32_t GW_OFF = GA_OFF + PG_ROWS * 4;             // schedule: block scan [16] int64, start int64, request, total
-constexpr uint32_t GB_OFF = GW_OFF + 16 * 8 + 32;
-constexpr int GB_KFULL = 0, GB_KFREE = 2, GB_SREADY = 4, GB_PREADY = 6, GB_PVDONE = 7, GB_QFREE = 8, GB_N = 9;
+constexpr uint32_t GX_OFF = GA_OFF + PG_ROWS * 4;             // [2][64] fp32: maxima, then sums, of the two halves of a block's rows
+constexpr uint32_t GW_OFF = GX_OFF + 2 * PG_ROWS * 4;         // schedule: block scan [20] int64, start int64, request
+constexpr uint32_t GB_OFF = GW_OFF + 22 * 8;
+// KFULL, KFREE: [2 stages][4 groups of dims]
+constexpr int GB_KFULL = 0, GB_KFREE = 8, GB_SREADY = 16, GB_SFREE = 18, GB_PREADY = 20, GB_PVDONE = 21, GB_QFREE = 22, GB_N = 23;
 constexpr uint32_t GMISC_OFF = GB_OFF + GB_N * 8;
 constexpr uint32_t G_SMEM = GMISC_OFF + 16 + 1024;
 static_assert(G_SMEM <= 227 * 1024, "shared memory budget");
@@ -55,7 +65,7 @@ static_assert(GB_OFF % 8 == 0 && GA_OFF % 16 == 0 && GW_OFF % 8 == 0, "alignment
 constexpr uint32_t GT_O = 0, GT_S = 256;          // tensor memory: dims block b of O^T at 64 b, the two score buffers at 256 and 320
 constexpr uint32_t G_DESC_HI = desc_hi(1024, (uint32_t)SWIZZLE_128B);
 
-enum { WP_KFULL = 61, WP_KFREE = 62, WP_SREADY = 63, WP_PREADY = 64, WP_PVDONE = 65, WP_QFREE = 66 };
+enum { WP_KFULL = 61, WP_KFREE = 62, WP_SREADY = 63, WP_PREADY = 64, WP_PVDONE = 65, WP_QFREE = 66, WP_SFREE = 67 };
 
 __device__ __forceinline__ uint32_t gswz(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
 
@@ -132,10 +142,11 @@ __device__ __forceinline__ void dequant16(uint4 v, float scale, uint32_t (&d)[8]
     }
 }
 
-template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_paged_kernel(const PagedParams p) {
-    constexpr bool F16 = LAYOUT == SMLA_LAYOUT_F16;
-    constexpr bool PACKED = LAYOUT == SMLA_LAYOUT_V32 || LAYOUT == SMLA_LAYOUT_MODEL1;
+template <int LAYOUT> __global__ void __launch_bounds__(paged_threads(LAYOUT), 1)
+attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map) {
+    constexpr bool F16 = LAYOUT == SMLA_LAYOUT_F16, PACKED = packed_rows(LAYOUT);
     constexpr int CHUNKS = LAYOUT == SMLA_LAYOUT_MODEL1 ? 8 : 9;
+    constexpr int LD0 = PG_SM_WARPS, S_WARP = LD0 + load_warps(LAYOUT), PV_WARP = S_WARP + 1, WARPS = paged_threads(LAYOUT) / 32;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -148,10 +159,13 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
     const int live = min(p.rows - row0, PG_ROWS);
 
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(GB_KFULL + i), PG_LD_WARPS / 2);
+        for (int i = 0; i < 8; ++i) {
+            mbar_init(bar(GB_KFULL + i), PACKED ? 4 : 1);
             mbar_init(bar(GB_KFREE + i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(bar(GB_SREADY + i), 1);
+            mbar_init(bar(GB_SFREE + i), PG_SM_WARPS);
         }
         mbar_init(bar(GB_PREADY), PG_SM_WARPS);
         mbar_init(bar(GB_PVDONE), 1);
@@ -160,13 +174,13 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
         for (int i = 0; i < 4; ++i) reinterpret_cast<volatile unsigned*>(sm + GN_OFF)[i] = 0u;
         mbar_init_fence();
     }
-    if (warp == PG_MMA_WARP) { tmem_alloc(base + GMISC_OFF, 512); tmem_relinquish(); }
+    if (warp == S_WARP) { tmem_alloc(base + GMISC_OFF, 512); tmem_relinquish(); }
     grid_dep_wait();
     grid_dep_launch();
 
     // ---- the partition's part of the line: every thread sums the requests of its share, the block scans the sums
     long long* scan = reinterpret_cast<long long*>(sm + GW_OFF);
-    const int per = (p.batch + PG_THREADS - 1) / PG_THREADS;
+    const int per = (p.batch + (int)blockDim.x - 1) / (int)blockDim.x;
     const int r_lo = min(tid * per, p.batch), r_hi = min(r_lo + per, p.batch);
     long long sum = 0;
     for (int r = r_lo; r < r_hi; ++r) sum += paged_blocks(paged_length(p, r)) + PG_START;
@@ -182,7 +196,7 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
     tc_fence_after();
     long long before = incl - sum, total = 0;
 #pragma unroll
-    for (int w = 0; w <= PG_MMA_WARP; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         if (w < warp) before += scan[w];
         total += scan[w];
     }
@@ -194,22 +208,29 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
             if (lo < before + w) break;
             before += w;
         }
-        scan[16] = before;
-        *reinterpret_cast<int*>(scan + 17) = r;
+        scan[20] = before;
+        *reinterpret_cast<int*>(scan + 21) = r;
     }
     __syncthreads();
-    Pieces piece(lo, hi, lo < hi ? *reinterpret_cast<int*>(scan + 17) : p.batch, lo < hi ? scan[16] : 0);
+    Pieces piece(lo, hi, lo < hi ? *reinterpret_cast<int*>(scan + 21) : p.batch, lo < hi ? scan[20] : 0);
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + GMISC_OFF);
+    if (PACKED) {
+        if (warp < PG_SM_WARPS) setmaxnreg_dec<PG_REGS_SOFTMAX>();
+        else if (warp < S_WARP) setmaxnreg_inc<PG_REGS_LOAD>();
+        else setmaxnreg_dec<PG_REGS_MMA>();
+    }
 
     if (warp < PG_SM_WARPS) {
         // =================================================================== softmax + epilogue
-        const int ra = 16 * warp + (lane >> 2), rb = ra + 8;      // the thread's query rows, columns 8 i + 2 (lane % 4) + {0, 1}
-        const int quad = lane & 3;
-        const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
+        // The thread's query rows ra and rb, and of a block's rows [32 half, +32) the columns 8 i + 2 (lane % 4) + {0, 1}.
+        const int quarter = warp & 3, half = warp >> 2, quad = lane & 3;
+        const int ra = 16 * quarter + (lane >> 2), rb = ra + 8;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
         const float c = p.sm_scale * LOG2E;
         float* factor = reinterpret_cast<float*>(sm + GA_OFF);
-        unsigned* none = reinterpret_cast<unsigned*>(sm + GN_OFF);           // [2 stages] 64 bits
-        const int cols = (live + 31) >> 5;                        // halves of 32 columns of O^T in use
+        float* other = reinterpret_cast<float*>(sm + GX_OFF);
+        unsigned* none = reinterpret_cast<unsigned*>(sm + GN_OFF);             // [2 stages] 64 bits
+        const int n = min(live - 32 * half, 32);                  // rows of O (columns of O^T) in the epilogue's half
         uint32_t it = 0;
         bool dead = false, stop = false;
         while (!stop && piece.next(p)) {
@@ -224,36 +245,39 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
             const int see_a = sees(ra), see_b = sees(rb), see_least = sees(0);
             float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
             for (int b = piece.b0; b < piece.b1; ++b, ++it) {
-                if (!dead) dead = !mbar_wait_lean(bar(GB_SREADY + (it & 1)), (it >> 1) & 1u, abort_addr, WP_SREADY);
-                uint32_t sv[32];
+                const uint32_t st = it & 1;
+                if (!dead) dead = !mbar_wait_lean(bar(GB_SREADY + st), (it >> 1) & 1u, abort_addr, WP_SREADY);
+                uint32_t sv[16];
                 float mx_a = -INFINITY, mx_b = -INFINITY;
                 const int pos0 = b * 64;
-                const bool tail = pos0 > see_least - 64;          // some row of the block is hidden from some query
+                unsigned long long valid = ~0ull;
                 bool odd = false;
                 if (!dead) {
                     tc_fence_after();
-                    tmem_ld_16x256b_x8(lane_addr + GT_S + 64 * (it & 1), sv);
-                    const unsigned long long valid = *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * (it & 1));
+                    tmem_ld_16x256b_x4(lane_addr + GT_S + 64 * st + 32 * half, sv);
+                    valid = *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * st);
                     tmem_wait_ld();
-                    if (valid == ~0ull && !tail) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(GB_SFREE + st));
+                    if (valid == ~0ull && pos0 <= see_least - 64) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * c);
+                        for (int i = 0; i < 16; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * c);
                     } else {
-                        unsigned bad[2] = {0u, 0u};
+                        unsigned bad = 0u;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int col = 8 * (i >> 2) + 2 * quad + (i & 1);
+                        for (int i = 0; i < 16; ++i) {
+                            const int col = 8 * (i >> 2) + 2 * quad + (i & 1), at = 32 * half + col;
                             const float x = __uint_as_float(sv[i]) * c;
-                            const bool there = (valid >> col) & 1, seen = there && pos0 + col < ((i & 2) ? see_b : see_a);
-                            if (there && !seen && !(fabsf(x) < INFINITY)) bad[col >> 5] |= 1u << (col & 31);
+                            const bool there = (valid >> at) & 1, seen = there && pos0 + at < ((i & 2) ? see_b : see_a);
+                            if (there && !seen && !(fabsf(x) < INFINITY)) bad |= 1u << col;
                             sv[i] = __float_as_uint(seen ? x : -INFINITY);
                         }
-                        if (bad[0]) atomicOr(none + 2 * (it & 1), bad[0]);
-                        if (bad[1]) atomicOr(none + 2 * (it & 1) + 1, bad[1]);
-                        odd = (bad[0] | bad[1]) != 0u;
+                        if (bad) atomicOr(none + 2 * st + half, bad);
+                        odd = bad != 0u;
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
+                    for (int i = 0; i < 16; i += 4) {
                         mx_a = fmaxf(mx_a, fmaxf(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])));
                         mx_b = fmaxf(mx_b, fmaxf(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])));
                     }
@@ -263,45 +287,48 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
                         mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, o));
                     }
                 }
-                const bool grow_a = mx_a > m_a + PG_TAU, grow_b = mx_b > m_b + PG_TAU;      // false while a row has seen nothing
-                const float al_a = grow_a ? ex2(m_a - mx_a) : 1.f, al_b = grow_b ? ex2(m_b - mx_b) : 1.f;
-                if (quad == 0) { factor[ra] = al_a; factor[rb] = al_b; }
-                if (named_bar_or(1, PG_SM_WARPS * 32, grow_a || grow_b || odd || dead || *abort_flag != 0)) {
-                    // rare: a maximum grows, a hidden row is no number, or the CTA gives up
-                    if (grow_a) { m_a = mx_a; l_a *= al_a; }
-                    if (grow_b) { m_b = mx_b; l_b *= al_b; }
-                    const unsigned long long hide = *reinterpret_cast<volatile unsigned long long*>(none + 2 * (it & 1));
-                    if (b > piece.b0 && !dead) {
-                        dead = !mbar_wait_lean(bar(GB_PVDONE), (it - 1) & 1u, abort_addr, WP_PVDONE);
+                if (quad == 0) { other[half * PG_ROWS + ra] = mx_a; other[half * PG_ROWS + rb] = mx_b; }
+                const bool grow = mx_a > m_a + PG_TAU || mx_b > m_b + PG_TAU;                // false while a row has seen nothing
+                if (named_bar_or(1, PG_SM_THREADS, grow || odd || dead || *abort_flag != 0) || valid != ~0ull) {
+                    // rare: a maximum grows, the request's last rows, a hidden row that is no number, or the CTA gives up
+                    const float all_a = fmaxf(other[ra], other[PG_ROWS + ra]), all_b = fmaxf(other[rb], other[PG_ROWS + rb]);
+                    float al_a = 1.f, al_b = 1.f;
+                    if (all_a > m_a + PG_TAU) { al_a = ex2(m_a - all_a); m_a = all_a; l_a *= al_a; }
+                    if (all_b > m_b + PG_TAU) { al_b = ex2(m_b - all_b); m_b = all_b; l_b *= al_b; }
+                    if (quad == 0 && half == 0) { factor[ra] = al_a; factor[rb] = al_b; }
+                    // Rows that are not there, and rows hidden from some query whose score is no number, would reach queries through
+                    // 0 x V: their values are taken out of the stage.  Queries that see such a row have a weight that is no number.
+                    const unsigned long long hide = ~valid | *reinterpret_cast<volatile unsigned long long*>(none + 2 * st);
+                    if (hide != 0ull && !dead) {
+                        for (int i = tid; i < 64 * CHUNKS * 8; i += PG_SM_THREADS) {
+                            const int r = (i >> 3) & 63;
+                            if ((hide >> r) & 1)
+                                *reinterpret_cast<uint4*>(sm + GK_OFF + st * G_STAGE + (i >> 9) * G_CHUNK + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    if (b > piece.b0 && !dead) dead = !mbar_wait_lean(bar(GB_PVDONE), (it - 1) & 1u, abort_addr, WP_PVDONE);
+                    if (named_bar_or(1, PG_SM_THREADS, dead || *abort_flag != 0)) { stop = true; break; }
+                    if (b > piece.b0 && n > 0) {
                         tc_fence_after();
 #pragma unroll 1
-                        for (int k = 0; k < 8; ++k) {
-                            if ((k & 1) >= cols) continue;
-                            uint32_t o[32];
-                            tmem_ld32(lane_addr + GT_O + 32 * k, o);
+                        for (int d = 0; d < 8; ++d) {
+                            const uint32_t at = lane_addr + GT_O + 64 * (d >> 1) + 32 * half + 16 * (d & 1);
+                            uint32_t o[16];
+                            tmem_ld16(at, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor[32 * (k & 1) + i]);
-                            tmem_st32(lane_addr + GT_O + 32 * k, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor[32 * half + 16 * (d & 1) + i]);
+                            tmem_st16(at, o);
                         }
                         tmem_wait_st();
                     }
-                    if (hide != 0ull) {
-                        // A row hidden from some query whose score is no number would reach that query through 0 x V: its values are
-                        // taken out of the stage.  Queries that see it have a weight that is no number.
-                        for (int i = tid; i < 64 * CHUNKS * 8; i += PG_SM_WARPS * 32) {
-                            const int r = (i >> 3) & 63;
-                            if ((hide >> r) & 1)
-                                *reinterpret_cast<uint4*>(sm + GK_OFF + (it & 1) * G_STAGE + (i >> 9) * G_CHUNK + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                    }
-                    if (named_bar_or(1, PG_SM_WARPS * 32, dead || *abort_flag != 0)) { stop = true; break; }
-                    if (tid == 0) *reinterpret_cast<volatile unsigned long long*>(none + 2 * (it & 1)) = 0ull;      // (next written two blocks from here)
+                    if (tid == 0) *reinterpret_cast<volatile unsigned long long*>(none + 2 * st) = 0ull;      // (next written two blocks from here)
+                    named_bar_sync(1, PG_SM_THREADS);             // the factors and maxima have been read
                 }
                 const float ma = m_a == -INFINITY ? 0.f : m_a, mb = m_b == -INFINITY ? 0.f : m_b;
-                uint32_t w[16];
+                uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     const float a0 = ex2(__uint_as_float(sv[4 * i]) - ma), a1 = ex2(__uint_as_float(sv[4 * i + 1]) - ma);
                     const float b0 = ex2(__uint_as_float(sv[4 * i + 2]) - mb), b1 = ex2(__uint_as_float(sv[4 * i + 3]) - mb);
                     l_a += a0 + a1;
@@ -312,9 +339,9 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
                 // the weights of the block before have been read
                 if (it > 0 && !dead) dead = !mbar_wait_lean(bar(GB_PVDONE), (it - 1) & 1u, abort_addr, WP_PVDONE);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    *reinterpret_cast<uint32_t*>(sm + GP_OFF + gswz((uint32_t)ra, (uint32_t)i) + 4 * quad) = w[2 * i];
-                    *reinterpret_cast<uint32_t*>(sm + GP_OFF + gswz((uint32_t)rb, (uint32_t)i) + 4 * quad) = w[2 * i + 1];
+                for (int i = 0; i < 4; ++i) {
+                    *reinterpret_cast<uint32_t*>(sm + GP_OFF + gswz((uint32_t)ra, (uint32_t)(4 * half + i)) + 4 * quad) = w[2 * i];
+                    *reinterpret_cast<uint32_t*>(sm + GP_OFF + gswz((uint32_t)rb, (uint32_t)(4 * half + i)) + 4 * quad) = w[2 * i + 1];
                 }
                 fence_proxy_async();
                 tc_fence_before();
@@ -330,10 +357,12 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
                 l_a += __shfl_xor_sync(0xffffffffu, l_a, o);
                 l_b += __shfl_xor_sync(0xffffffffu, l_b, o);
             }
+            if (quad == 0) { other[half * PG_ROWS + ra] = l_a; other[half * PG_ROWS + rb] = l_b; }
+            if (named_bar_or(1, PG_SM_THREADS, dead || *abort_flag != 0)) { stop = true; break; }
             const size_t rec = whole ? (size_t)piece.req : (size_t)(2 * part + (piece.b0 == 0 ? 1 : 0));
-            if (quad < 2) {                                       // one lane for each of the quad's rows
+            if (half == 0 && quad < 2) {                          // one lane for each of the quad's rows
                 const int r = quad == 0 ? ra : rb;
-                const float l = quad == 0 ? l_a : l_b, m = quad == 0 ? m_a : m_b;
+                const float l = other[r] + other[PG_ROWS + r], m = quad == 0 ? m_a : m_b;
                 float lse = l == 0.f ? NEG_BIG : log2f(l) + m, denom = l;
                 if (r < live) {
                     if (whole && p.attn_sink != nullptr) {
@@ -345,91 +374,137 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
                 }
                 factor[r] = l == 0.f ? 0.f : 1.f / denom;         // 0: nothing is seen, or the sink takes all
             }
-            if (named_bar_or(1, PG_SM_WARPS * 32, dead || *abort_flag != 0)) { stop = true; break; }
+            named_bar_sync(1, PG_SM_THREADS);
+            if (n > 0) {
 #pragma unroll 1
-            for (int k = 0; k < 8; ++k) {
-                if ((k & 1) >= cols) continue;
-                uint32_t o[32];
-                if (piece.b1 > piece.b0) tmem_ld32(lane_addr + GT_O + 32 * k, o);
-                tmem_wait_ld();
-                const size_t at = (rec * p.rows + row0 + 32 * (k & 1)) * D_V + 128 * (k >> 1) + 32 * warp + lane;
-                const int n = min(live - 32 * (k & 1), 32);
+                for (int d = 0; d < 8; ++d) {
+                    const int r0 = 32 * half + 16 * (d & 1);
+                    uint32_t o[16];
+                    if (piece.b1 > piece.b0) tmem_ld16(lane_addr + GT_O + 64 * (d >> 1) + r0, o);
+                    tmem_wait_ld();
+                    const size_t at = (rec * p.rows + row0 + r0) * D_V + 128 * (d >> 1) + 32 * quarter + lane;
+                    uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+                    float* part_out = p.o_part + at;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float f = factor[32 * (k & 1) + i], v = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
-                    if (i < n) {
-                        if (whole) static_cast<uint16_t*>(p.out)[at + (size_t)i * D_V] = out_bits<F16>(v);
-                        else p.o_part[at + (size_t)i * D_V] = v;
+                    for (int i = 0; i < 16; ++i) {
+                        const float f = factor[r0 + i], v = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
+                        if (r0 + i < live) {
+                            if (whole) out[i * D_V] = out_bits<F16>(v);
+                            else part_out[i * D_V] = v;
+                        }
                     }
                 }
             }
             tc_fence_before();
-            named_bar_sync(1, PG_SM_WARPS * 32);                  // the factors have been read
+            named_bar_sync(1, PG_SM_THREADS);                     // the factors have been read
         }
-    } else if (warp < PG_MMA_WARP) {
+    } else if (warp < S_WARP) {
         // =================================================================== rows into the stages, and the queries
-        const int stage = (warp - PG_SM_WARPS) >> 2, gw = (warp - PG_SM_WARPS) & 3;
-        const uint32_t kst = GK_OFF + stage * G_STAGE;
         uint32_t it = 0, pieces = 0;
         bool ok = true;
-        while (ok && piece.next(p)) {
-            if (piece.b1 == piece.b0) continue;
-            const int32_t* table = p.table + (int64_t)piece.req * p.table_stride;
-            for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
-                if ((it & 1) != (uint32_t)stage) continue;
-                // where row r of the block lies: its page (null: no entry) and its place in there
-                auto row_at = [&](int r, int& in) -> const uint8_t* {
-                    const int pos = b * 64 + r;
-                    in = 0;
-                    if (pos >= piece.len) return nullptr;
-                    const int j = pos / p.page_block_size, page = ld_in(table + j);
-                    if (page < 0 || page >= p.num_pages) return nullptr;
-                    in = pos - j * p.page_block_size;
-                    return p.cache + (int64_t)page * p.page_stride;
-                };
-                unsigned bits = 0u;
-                int in;
-                if constexpr (!PACKED) {
-                    const uint8_t* src[4];
+        if constexpr (!PACKED) {
+            // A warp per group of dims: a copy takes its warp about 130 cycles to issue, all of them from one warp 3900 cycles a block.
+            const int rows = p.copy_rows, copies = 64 / rows;     // rows of a copy, copies of a block (and chunk): lane i sees to i and i + 32
+            const int g = warp - LD0, c0 = 2 * g, c1 = g == 3 ? CHUNKS : c0 + 2;
+            int page[2], in[2];
+            unsigned v_lo, v_hi;                                  // rows that are there
+            uint32_t bytes;                                       // of a chunk
+            auto places = [&](int b) {                            // where block b's rows lie
+                unsigned long long valid = 0ull;
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        src[h] = row_at(16 * gw + 4 * h + (lane >> 3), in);
-                        const unsigned v = __ballot_sync(0xffffffffu, src[h] != nullptr);
-                        bits |= ((v & 1u) | ((v >> 7) & 2u) | ((v >> 14) & 4u) | ((v >> 21) & 8u)) << (4 * h);
-                        if (src[h] != nullptr) src[h] += (int64_t)in * (2 * D_QK) + (lane & 7) * 16;
-                    }
-                    if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + stage), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
-                    if (!ok) break;
-#pragma unroll
-                    for (int ch = 0; ch < CHUNKS; ++ch) {
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const bool there = src[h] != nullptr;
-                            cp_async16(base + kst + ch * G_CHUNK + gswz((uint32_t)(16 * gw + 4 * h + (lane >> 3)), lane & 7),
-                                       there ? src[h] + ch * 128 : p.q, there ? 16u : 0u);
+                for (int u = 0; u < 2; ++u) {
+                    const int i = lane + 32 * u, pos = b * 64 + i * rows;
+                    page[u] = -1;
+                    in[u] = 0;
+                    if (i < copies && pos < piece.len) {
+                        const int j = pos / p.page_block_size, e = ld_in(p.table + (int64_t)piece.req * p.table_stride + j);
+                        if (e >= 0 && e < p.num_pages) {
+                            page[u] = e;
+                            in[u] = pos - j * p.page_block_size;
+                            const int k = min(piece.len - pos, rows);
+                            valid |= (k == 64 ? ~0ull : (1ull << k) - 1ull) << (i * rows);
                         }
                     }
-                } else {
-                    constexpr int NOPE = LAYOUT == SMLA_LAYOUT_V32 ? D_NOPE : 448;
-                    constexpr int ROPE_AT = LAYOUT == SMLA_LAYOUT_V32 ? ROPE_OFF : 448;
-                    const uint8_t* mine = row_at(16 * gw + (lane & 15), in);       // lane i: row i % 16 of the warp
-                    bits = __ballot_sync(0xffffffffu, mine != nullptr) & 0xffffu;
-                    uint2 sc8 = make_uint2(0u, 0u);
+                }
+                v_lo = __reduce_or_sync(0xffffffffu, (unsigned)valid);
+                v_hi = __reduce_or_sync(0xffffffffu, (unsigned)(valid >> 32));
+                bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, page[0] >= 0)) + __popc(__ballot_sync(0xffffffffu, page[1] >= 0))) * rows * 128u;
+            };
+            int b = 0;
+            bool first = true;
+            auto advance = [&](bool inside) {                     // to the next block
+                first = false;
+                if (inside && ++b < piece.b1) return true;
+                do {
+                    if (!piece.next(p)) return false;
+                } while (piece.b1 == piece.b0);
+                b = piece.b0;
+                first = true;
+                return true;
+            };
+            bool have = advance(false);
+            if (have) places(b);
+            for (; have && ok; ++it) {
+                const uint32_t st = it & 1, full = bar(GB_KFULL + 4 * st + g);
+                if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + 4 * st + g), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
+                if (ok && first && pieces > 0) ok = mbar_wait_lean(bar(GB_QFREE), (pieces - 1) & 1u, abort_addr, WP_QFREE);
+                if (!ok) break;
+                if (g == 0 && lane == 0) *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * st) = ((unsigned long long)v_hi << 32) | v_lo;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(full, (uint32_t)(c1 - c0) * (bytes + (first ? G_CHUNK : 0u)));
+                    if (first)
+                        for (int ch = c0; ch < c1; ++ch) tma_load_2d(base + GQ_OFF + ch * G_CHUNK, &q_map, ch * 64, piece.req * p.rows + row0, full);
+                }
+#pragma unroll 1
+                for (int i = 0; i < copies; ++i) {                // (under elect_one, with operands that are the same in all lanes)
+                    const int e = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31), y = __shfl_sync(0xffffffffu, i < 32 ? in[0] : in[1], i & 31);
+                    if (e >= 0 && elect_one())
+                        for (int ch = c0; ch < c1; ++ch)
+                            tma_load_3d(base + GK_OFF + st * G_STAGE + ch * G_CHUNK + i * rows * 128, &k_map, ch * 64, y, e, full);
+                }
+                __syncwarp();
+                if (first) ++pieces;
+                have = advance(true);
+                if (have) places(b);                              // read while the stage is in use
+            }
+        } else {
+            const int stage = (warp - LD0) >> 2, gw = (warp - LD0) & 3;
+            const uint32_t kst = GK_OFF + stage * G_STAGE;
+            constexpr int NOPE = LAYOUT == SMLA_LAYOUT_V32 ? D_NOPE : 448;
+            constexpr int ROPE_AT = LAYOUT == SMLA_LAYOUT_V32 ? ROPE_OFF : 448;
+            while (ok && piece.next(p)) {
+                if (piece.b1 == piece.b0) continue;
+                const int32_t* table = p.table + (int64_t)piece.req * p.table_stride;
+                for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
+                    if ((it & 1) != (uint32_t)stage) continue;
+                    // lane i: where row i % 16 of the warp's lies (0: no entry)
                     unsigned long long at = 0ull;
-                    if (mine != nullptr) {
-                        if (LAYOUT == SMLA_LAYOUT_MODEL1)
-                            sc8 = ld_in(reinterpret_cast<const uint2*>(mine + (int64_t)p.page_block_size * SMLA_M1_DATA_BYTES + (int64_t)in * 8));
-                        at = reinterpret_cast<unsigned long long>(mine + (int64_t)in * (LAYOUT == SMLA_LAYOUT_V32 ? ROW_BYTES : SMLA_M1_DATA_BYTES));
+                    uint2 sc8 = make_uint2(0u, 0u);
+                    const int pos = b * 64 + 16 * gw + (lane & 15);
+                    if (pos < piece.len) {
+                        const int j = pos / p.page_block_size, page = ld_in(table + j), in = pos - j * p.page_block_size;
+                        if (page >= 0 && page < p.num_pages) {
+                            const uint8_t* mine = p.cache + (int64_t)page * p.page_stride;
+                            if (LAYOUT == SMLA_LAYOUT_MODEL1)
+                                sc8 = ld_in(reinterpret_cast<const uint2*>(mine + (int64_t)p.page_block_size * SMLA_M1_DATA_BYTES + (int64_t)in * 8));
+                            at = reinterpret_cast<unsigned long long>(mine + (int64_t)in * (LAYOUT == SMLA_LAYOUT_V32 ? ROW_BYTES : SMLA_M1_DATA_BYTES));
+                        }
                     }
+                    const unsigned bits = __ballot_sync(0xffffffffu, at != 0ull) & 0xffffu;
                     uint4 nope[16], rope[4];
-                    float scale[16];
+                    float scale[2] = {0.f, 0.f};                  // of row lane / 4 (+ 8), block lane % 4 of 128 dims
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, at, i));
                         nope[i] = make_uint4(0, 0, 0, 0);
-                        scale[i] = 0.f;
                         if (src != nullptr && lane < NOPE / 16) nope[i] = ld_in_once(reinterpret_cast<const uint4*>(src) + lane);
-                        if (LAYOUT == SMLA_LAYOUT_V32 && src != nullptr) scale[i] = ld_in(reinterpret_cast<const float*>(src + SCALE_OFF) + (lane >> 3));
+                    }
+                    if (LAYOUT == SMLA_LAYOUT_V32) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, at, (lane >> 2) + 8 * u));
+                            if (src != nullptr) scale[u] = ld_in(reinterpret_cast<const float*>(src + SCALE_OFF) + (lane & 3));
+                        }
                     }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
@@ -437,15 +512,28 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
                         rope[u] = make_uint4(0, 0, 0, 0);
                         if (src != nullptr) rope[u] = ld_in_once(reinterpret_cast<const uint4*>(src + ROPE_AT) + (lane & 7));
                     }
-                    if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + stage), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
+                    if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + 4 * stage + 3), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
                     if (!ok) break;
+                    const uint32_t full = bar(GB_KFULL + 4 * stage);
+                    const bool queries = b == piece.b0 && gw == 0;       // the piece's queries come with its first block
+                    if (queries) {
+                        if (pieces > 0) ok = mbar_wait_lean(bar(GB_QFREE), (pieces - 1) & 1u, abort_addr, WP_QFREE);
+                        if (!ok) break;
+                        if (elect_one()) {
+                            mbar_expect_tx(full, CHUNKS * G_CHUNK);
+                            for (int ch = 0; ch < CHUNKS; ++ch) tma_load_2d(base + GQ_OFF + ch * G_CHUNK, &q_map, ch * 64, piece.req * p.rows + row0, full);
+                        }
+                        __syncwarp();
+                    }
                     const uint32_t chunk = kst + (lane >> 2) * G_CHUNK;
                     const bool swap = (lane & 4) != 0;           // neighbouring chunks store their two pieces in opposite order: no bank conflicts
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const uint32_t r = (uint32_t)(16 * gw + i), pc = 2u * (lane & 3);
-                        float f = scale[i];
-                        if (LAYOUT == SMLA_LAYOUT_MODEL1) {
+                        float f;
+                        if (LAYOUT == SMLA_LAYOUT_V32) {
+                            f = __shfl_sync(0xffffffffu, scale[i >> 3], 4 * (i & 7) + (lane >> 3));
+                        } else {
                             const uint32_t w0 = __shfl_sync(0xffffffffu, sc8.x, i), w1 = __shfl_sync(0xffffffffu, sc8.y, i);
                             f = __uint_as_float(((((lane & 16) ? w1 : w0) >> (8 * ((lane >> 2) & 3))) & 0xffu) << 23);
                         }
@@ -460,105 +548,78 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         *reinterpret_cast<uint4*>(sm + kst + (CHUNKS - 1) * G_CHUNK + gswz((uint32_t)(16 * gw + 4 * u + (lane >> 3)), lane & 7)) = rope[u];
+                    if (lane == 0) *reinterpret_cast<volatile uint16_t*>(sm + GV_OFF + 8 * stage + 2 * gw) = (uint16_t)bits;
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full);
                 }
-                if (b == piece.b0) {                              // the piece's queries come with its first block
-                    if (pieces > 0) ok = mbar_wait_lean(bar(GB_QFREE), (pieces - 1) & 1u, abort_addr, WP_QFREE);
-                    if (!ok) break;
-                    const uint8_t* q = p.q + ((size_t)piece.req * p.rows + row0) * (CHUNKS * 128);
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const int r = 16 * gw + 4 * h + (lane >> 3);
-                        const bool there = r < live;
-                        const uint8_t* at = there ? q + (size_t)r * (CHUNKS * 128) + (lane & 7) * 16 : p.q;
-#pragma unroll
-                        for (int ch = 0; ch < CHUNKS; ++ch)
-                            cp_async16(base + GQ_OFF + ch * G_CHUNK + gswz((uint32_t)r, lane & 7), at + (there ? ch * 128 : 0), there ? 16u : 0u);
-                    }
-                }
-                cp_async_wait_all();
-                if (lane == 0) *reinterpret_cast<volatile uint16_t*>(sm + GV_OFF + 8 * stage + 2 * gw) = (uint16_t)bits;
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(GB_KFULL + stage));
+                ++pieces;
             }
-            ++pieces;
         }
-    } else {
-        // =================================================================== MMA issue
-        const uint32_t idesc_s = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, false, false, 64, 64);
-        const uint32_t idesc_o = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, true, false, 128, (uint32_t)((live + 15) & ~15));
+    } else if (warp == S_WARP) {
+        // =================================================================== scores
+        const uint32_t idesc = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, false, false, 64, 64);
         const uint32_t q_lo = desc_lo(base + GQ_OFF, 16), k_lo = desc_lo(base + GK_OFF, 16);
-        const uint32_t v_lo = desc_lo(base + GK_OFF, G_CHUNK), p_lo = desc_lo(base + GP_OFF, 16);      // V MN-major: the next 64 dims lie a chunk further
-        uint32_t scored = 0, done = 0, firsts = 0;                // blocks whose scores / whose P.V have been issued; bit i: block i % 2 is its piece's first
-        bool ok = true, have = false;
-        int b = 0;
-        auto advance = [&]() {                                    // to the next block
-            if (have && ++b < piece.b1) return;
-            do { have = piece.next(p); } while (have && piece.b1 == piece.b0);
-            b = piece.b0;
-        };
-        advance();
-        while (ok && (have || done < scored)) {
-            // scores run at most one block ahead of P.V (their buffer, and the order in which stages become free)
-            const bool may_score = have && scored - done <= 1;
-            bool score = false;
-            if (may_score && scored == done) {
-                ok = mbar_wait_lean(bar(GB_KFULL + (scored & 1)), (scored >> 1) & 1u, abort_addr, WP_KFULL);
-                score = true;
-            } else {
-                // whichever is ready first: the next block's rows or this one's weights
-                uint32_t left = 1u << 26;
-                while (true) {
-                    if (may_score && __all_sync(0xffffffffu, mbar_test(bar(GB_KFULL + (scored & 1)), (scored >> 1) & 1u))) { score = true; break; }
-                    if (__all_sync(0xffffffffu, mbar_test(bar(GB_PREADY), done & 1u))) break;
-                    if (--left == 0u) { ok = mbar_wait_lean(bar(GB_PREADY), done & 1u, abort_addr, WP_PREADY); break; }
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && piece.next(p)) {
+            for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
+                const uint32_t st = it & 1;
+                if (it >= 2) ok = mbar_wait_lean(bar(GB_SFREE + st), ((it >> 1) - 1) & 1u, abort_addr, WP_SFREE);
+#pragma unroll 1
+                for (int g = 0; g < 4 && ok; ++g) {
+                    if (!PACKED || g == 0) ok = mbar_wait_lean(bar(GB_KFULL + 4 * st + g), (it >> 1) & 1u, abort_addr, WP_KFULL);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll 1
+                        for (int ch = 2 * g; ch < (g == 3 ? CHUNKS : 2 * g + 2); ++ch) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_f16(tmem + GT_S + 64 * st, make_desc(q_lo + ((ch * G_CHUNK + k * 32) >> 4), G_DESC_HI),
+                                        make_desc(k_lo + ((st * G_STAGE + ch * G_CHUNK + k * 32) >> 4), G_DESC_HI), idesc, (ch | k) != 0);
+                        }
+                        if (g == 3) {
+                            tc_commit(bar(GB_SREADY + st));
+                            if (b + 1 == piece.b1) tc_commit(bar(GB_QFREE));
+                        }
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok) break;
-            tc_fence_after();
-            if (score) {
-                const uint32_t st = scored & 1;
-                firsts = (firsts & ~(1u << st)) | ((b == piece.b0 ? 1u : 0u) << st);
-                const bool last = b + 1 == piece.b1;
+        }
+    } else if (warp == PV_WARP) {
+        // =================================================================== P.V
+        const uint32_t idesc = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, true, false, 128, (uint32_t)((live + 15) & ~15));
+        const uint32_t v_lo = desc_lo(base + GK_OFF, G_CHUNK), p_lo = desc_lo(base + GP_OFF, 16);      // V MN-major: the next 64 dims lie a chunk further
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && piece.next(p)) {
+            for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
+                const uint32_t st = it & 1;
+                ok = mbar_wait_lean(bar(GB_PREADY), it & 1u, abort_addr, WP_PREADY);
+                if (!ok) break;
+                tc_fence_after();
                 if (elect_one()) {
 #pragma unroll 1
-                    for (int ch = 0; ch < CHUNKS; ++ch) {
+                    for (int d = 0; d < 4; ++d) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_f16(tmem + GT_S + 64 * st, make_desc(q_lo + ((ch * G_CHUNK + k * 32) >> 4), G_DESC_HI),
-                                    make_desc(k_lo + ((st * G_STAGE + ch * G_CHUNK + k * 32) >> 4), G_DESC_HI), idesc_s, (ch | k) != 0);
-                    }
-                    tc_commit(bar(GB_SREADY + st));
-                    if (last) tc_commit(bar(GB_QFREE));
-                }
-                __syncwarp();
-                ++scored;
-                advance();
-            } else {
-                const uint32_t st = done & 1;
-                const bool first = (firsts >> st) & 1u;
-                if (elect_one()) {
-#pragma unroll 1
-                    for (int k = 0; k < 4; ++k) {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
                             mma_f16(tmem + GT_O + 64 * d, make_desc(v_lo + ((st * G_STAGE + 2 * d * G_CHUNK + k * 2048) >> 4), G_DESC_HI),
-                                    make_desc(p_lo + ((k * 32) >> 4), G_DESC_HI), idesc_o, !first || k != 0);
+                                    make_desc(p_lo + ((k * 32) >> 4), G_DESC_HI), idesc, b != piece.b0 || k != 0);
+                        tc_commit(bar(GB_KFREE + 4 * st + d));
                     }
-                    tc_commit(bar(GB_KFREE + st));
                     tc_commit(bar(GB_PVDONE));
                 }
                 __syncwarp();
-                ++done;
             }
         }
     }
 
-    if (*abort_flag != 0) {        // a wait gave up: MMAs may still be in flight; give them time to finish
+    if (*abort_flag != 0) {        // a wait gave up: copies and MMAs may still be in flight; give them time to finish
         const long long t0 = clock64();
         while (clock64() - t0 < 200000) { }
     }
-    cp_async_wait_all();
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && *abort_flag != 0 && p.status != nullptr) {
@@ -566,27 +627,41 @@ template <int LAYOUT> __global__ void __launch_bounds__(PG_THREADS, 1) attn_page
         atomicAdd(p.status + 1, 1);
         p.status[2] = blockIdx.x;
     }
-    if (warp == PG_MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+    if (warp == S_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// One warp per query row of a request: joins what its partitions left, in their order.  Requests within one partition are done.
-template <bool F16> __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p) {
+// Four warps per query row of a request: join what its partitions left.  Requests within one partition are done.  Warp w sums records w,
+// w + 4, ..., four of them asked for at a time: the merge is a chain of latencies (one request of 131072 rows in 74 partitions: 64 us with one
+// warp per row and a record at a time).  The order of the sums is fixed.
+constexpr int PC_WARPS = 4, PC_AHEAD = 4;
+template <bool F16> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combine_kernel(const PagedParams p) {
+    __shared__ float4 sums[PC_WARPS - 1][D_V / 4];
     grid_dep_wait();
     grid_dep_launch();
-    const int lane = threadIdx.x & 31;
-    const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (id >= (int64_t)p.batch * p.rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t id = blockIdx.x;
     const int req = (int)(id / p.rows), row = (int)(id - (int64_t)req * p.rows);
     const uint2 span = ld_in(reinterpret_cast<const uint2*>(p.spans + req));
     const int c0 = (int)span.x, n = (int)span.y - c0 + 1;
     if (n <= 1) return;
     auto record = [&](int s) { return (size_t)(s == 0 ? 2 * c0 + 1 : 2 * (c0 + s)) * p.rows + row; };
+    float4 v[PC_AHEAD][4];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < PC_AHEAD; ++u)
+            if (s0 + PC_WARPS * u < n) {
+                const float4* src = reinterpret_cast<const float4*>(p.o_part + record(s0 + PC_WARPS * u) * D_V) + lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[u][i] = ld_in_once(src + 32 * i);
+            }
+    };
+    load(warp);
     float mx = NEG_BIG, sum = 0.f;
     for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ld_in(p.lse_part + record(s)));
     mx = warp_max(mx);
     for (int s = lane; s < n; s += 32) {
-        const float v = ld_in(p.lse_part + record(s));
-        sum += v == NEG_BIG ? 0.f : exp2f(v - mx);
+        const float x = ld_in(p.lse_part + record(s));
+        sum += x == NEG_BIG ? 0.f : exp2f(x - mx);
     }
     sum = warp_sum(sum);
     float lse = sum == 0.f ? NEG_BIG : log2f(sum) + mx, denom = sum;
@@ -599,20 +674,38 @@ template <bool F16> __global__ void __launch_bounds__(256) paged_combine_kernel(
     float4 acc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < n; ++s) {
-        const size_t r = record(s);
-        const float v = ld_in(p.lse_part + r), w = v == NEG_BIG ? 0.f : exp2f(v - mx) * inv;
+    for (int s0 = warp; s0 < n; s0 += PC_WARPS * PC_AHEAD) {
+        if (s0 > warp) load(s0);
+#pragma unroll
+        for (int u = 0; u < PC_AHEAD; ++u) {
+            const int s = s0 + PC_WARPS * u;
+            if (s >= n) break;
+            const float x = ld_in(p.lse_part + record(s)), w = x == NEG_BIG ? 0.f : exp2f(x - mx) * inv;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[i].x += w * v[u][i].x; acc[i].y += w * v[u][i].y; acc[i].z += w * v[u][i].z; acc[i].w += w * v[u][i].w;
+            }
+        }
+    }
+    if (warp > 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[warp - 1][32 * i + lane] = acc[i];
+    }
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 0; w < PC_WARPS - 1; ++w) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float4 x = ld_in_once(reinterpret_cast<const float4*>(p.o_part + r * D_V + i * 128 + lane * 4));
-            acc[i].x += w * x.x; acc[i].y += w * x.y; acc[i].z += w * x.z; acc[i].w += w * x.w;
+            const float4 x = sums[w][32 * i + lane];
+            acc[i].x += x.x; acc[i].y += x.y; acc[i].z += x.z; acc[i].w += x.w;
         }
     }
     if (lane == 0) p.lse[id] = lse;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint2 v = make_uint2(pack_weights<F16>(acc[i].x, acc[i].y), pack_weights<F16>(acc[i].z, acc[i].w));
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (size_t)id * D_V + i * 128 + lane * 4) = v;
+        const uint2 r = make_uint2(pack_weights<F16>(acc[i].x, acc[i].y), pack_weights<F16>(acc[i].z, acc[i].w));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (size_t)id * D_V + i * 128 + lane * 4) = r;
     }
 }
 
@@ -628,30 +721,46 @@ int paged_parts(int batch, int rows, int pages_per_request, int page_block_size,
     return worth < most ? (int)(worth > 0 ? worth : 1) : most;
 }
 
-int launch_attn_paged(const PagedParams& p, int layout, cudaStream_t stream) {
-    typedef void (*Kernel)(const PagedParams);
-    static const Kernel kernels[4] = {attn_paged_kernel<SMLA_LAYOUT_V32>, attn_paged_kernel<SMLA_LAYOUT_MODEL1>, attn_paged_kernel<SMLA_LAYOUT_BF16>,
-                                      attn_paged_kernel<SMLA_LAYOUT_F16>};
+int launch_attn_paged(PagedParams p, int layout, cudaStream_t stream) {
+    typedef void (*Kernel)(const PagedParams, const CUtensorMap, const CUtensorMap);
     static std::atomic<bool> attr_set[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return set_error(SMLA_E_SHAPE, "attn_paged_kernel: device ordinal %d not supported", dev);
     if (!attr_set[dev]) {
-        for (const Kernel k : kernels) {
-            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G_SMEM);
+        const Kernel kernels[4] = {attn_paged_kernel<SMLA_LAYOUT_V32>, attn_paged_kernel<SMLA_LAYOUT_MODEL1>, attn_paged_kernel<SMLA_LAYOUT_BF16>,
+                                   attn_paged_kernel<SMLA_LAYOUT_F16>};
+        for (int i = 0; i < 4; ++i) {
+            cudaFuncAttributes fa;
+            if (i < 2 && (cudaFuncGetAttributes(&fa, kernels[i]) != cudaSuccess || fa.numRegs != PG_REGS_LAUNCH))
+                return set_error(SMLA_E_DEVICE, "attn_paged_kernel: compiled with %d registers per thread, the warpgroup budgets assume %d", fa.numRegs, PG_REGS_LAUNCH);
+            const cudaError_t e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G_SMEM);
             if (e != cudaSuccess) return set_error((int)e, "attn_paged_kernel: cannot reserve %u bytes of shared memory: %s", G_SMEM, cudaGetErrorString(e));
         }
         attr_set[dev] = true;
+    }
+    CUtensorMap q_map{}, k_map{};
+    const bool packed = packed_rows(layout), f16 = layout == SMLA_LAYOUT_F16;
+    const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint64_t d = layout == SMLA_LAYOUT_MODEL1 ? SMLA_M1_D_QK : D_QK;
+    const uint64_t q_dims[2] = {d, (uint64_t)p.batch * p.rows}, q_strides[1] = {2 * d};
+    const uint32_t q_box[2] = {64, PG_ROWS};
+    if (int e = encode_map(&q_map, type, 2, p.q, q_dims, q_strides, q_box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
+    p.copy_rows = 64;                              // the largest power of two that divides pages and blocks
+    while (p.page_block_size % p.copy_rows != 0) p.copy_rows >>= 1;
+    if (!packed && p.num_pages > 0) {
+        const uint64_t k_dims[3] = {D_QK, (uint64_t)p.page_block_size, (uint64_t)p.num_pages}, k_strides[2] = {2 * D_QK, (uint64_t)p.page_stride};
+        const uint32_t k_box[3] = {64, (uint32_t)p.copy_rows, 1};
+        if (int e = encode_map(&k_map, type, 3, p.cache, k_dims, k_strides, k_box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
     }
     const Kernel kernel = layout == SMLA_LAYOUT_V32      ? attn_paged_kernel<SMLA_LAYOUT_V32>
                           : layout == SMLA_LAYOUT_MODEL1 ? attn_paged_kernel<SMLA_LAYOUT_MODEL1>
                           : layout == SMLA_LAYOUT_BF16   ? attn_paged_kernel<SMLA_LAYOUT_BF16>
                                                          : attn_paged_kernel<SMLA_LAYOUT_F16>;
-    launch_dependent(kernel, dim3(p.num_parts, (p.rows + PG_ROWS - 1) / PG_ROWS), dim3(PG_THREADS), G_SMEM, stream, p);
+    launch_dependent(kernel, dim3(p.num_parts, (p.rows + PG_ROWS - 1) / PG_ROWS), dim3(paged_threads(layout)), G_SMEM, stream, p, q_map, k_map);
     if (int e = check_launch("attn_paged_kernel")) return e;
     if (p.num_parts == 1) return 0;                // every request is whole
-    const int64_t blocks = ((int64_t)p.batch * p.rows + 7) / 8;
-    launch_dependent(layout == SMLA_LAYOUT_F16 ? paged_combine_kernel<true> : paged_combine_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    launch_dependent(f16 ? paged_combine_kernel<true> : paged_combine_kernel<false>, dim3((unsigned)p.batch * (unsigned)p.rows), dim3(PC_WARPS * 32), 0, stream, p);
     return check_launch("paged_combine_kernel");
 }
 

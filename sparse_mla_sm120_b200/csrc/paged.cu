@@ -76,7 +76,8 @@ __device__ __forceinline__ int paged_length(const PagedParams& p, int req) {
 }
 __device__ __forceinline__ int paged_blocks(int len) { return (int)(((unsigned)len + 63u) >> 6); }
 __host__ __device__ __forceinline__ long long paged_share(long long total, int parts) {
-    const long long u = (total + parts - 1) / parts;
+    // (a 64-bit division takes hundreds of cycles)
+    const long long u = total + parts <= 0xffffffffll ? (long long)((unsigned)(total + parts - 1) / (unsigned)parts) : (total + parts - 1) / parts;
     return u > PG_START + PG_LEAST ? u : PG_START + PG_LEAST;
 }
 
@@ -230,13 +231,14 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
         float* factor = reinterpret_cast<float*>(sm + GA_OFF);
         float* other = reinterpret_cast<float*>(sm + GX_OFF);
         unsigned* none = reinterpret_cast<unsigned*>(sm + GN_OFF);             // [2 stages] 64 bits
-        const int n = min(live - 32 * half, 32);                  // rows of O (columns of O^T) in the epilogue's half
+        const bool busy = live > 32 * half;                       // the half has columns of O^T
         uint32_t it = 0;
         bool dead = false, stop = false;
         while (!stop && piece.next(p)) {
             const bool whole = piece.whole();
             if (row0 == 0 && tid == 0 && piece.b0 == 0) {
-                const int last = piece.nb == 0 ? part : (int)((piece.start + PG_START + piece.nb - 1) / share);
+                const long long end = piece.start + PG_START + piece.nb - 1;
+                const int last = whole ? part : (int)(end <= 0xffffffffll && share <= end ? (unsigned)end / (unsigned)share : end / share);
                 p.spans[piece.req] = make_int2(part, last);
             }
             // rows that query rows see: all of the request's, or up to the query's own
@@ -308,7 +310,7 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                     }
                     if (b > piece.b0 && !dead) dead = !mbar_wait_lean(bar(GB_PVDONE), (it - 1) & 1u, abort_addr, WP_PVDONE);
                     if (named_bar_or(1, PG_SM_THREADS, dead || *abort_flag != 0)) { stop = true; break; }
-                    if (b > piece.b0 && n > 0) {
+                    if (b > piece.b0 && busy) {
                         tc_fence_after();
 #pragma unroll 1
                         for (int d = 0; d < 8; ++d) {
@@ -375,25 +377,35 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 factor[r] = l == 0.f ? 0.f : 1.f / denom;         // 0: nothing is seen, or the sink takes all
             }
             named_bar_sync(1, PG_SM_THREADS);
-            if (n > 0) {
+            // 16 query rows at a time: their factors, then their 128 dims of the warp's lanes from all four accumulators
 #pragma unroll 1
-                for (int d = 0; d < 8; ++d) {
-                    const int r0 = 32 * half + 16 * (d & 1);
-                    uint32_t o[16];
-                    if (piece.b1 > piece.b0) tmem_ld16(lane_addr + GT_O + 64 * (d >> 1) + r0, o);
-                    tmem_wait_ld();
-                    const size_t at = (rec * p.rows + row0 + r0) * D_V + 128 * (d >> 1) + 32 * quarter + lane;
-                    uint16_t* out = static_cast<uint16_t*>(p.out) + at;
-                    float* part_out = p.o_part + at;
+            for (int r0 = 32 * half; r0 < min(live, 32 * half + 32); r0 += 16) {
+                float f[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float f = factor[r0 + i], v = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
-                        if (r0 + i < live) {
-                            if (whole) out[i * D_V] = out_bits<F16>(v);
-                            else part_out[i * D_V] = v;
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(factor + r0 + i);
+                    f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+                }
+                const size_t at = (rec * p.rows + row0 + r0) * D_V + 32 * quarter + lane;
+                const int left = live - r0;
+                auto store = [&](auto* dst, auto cvt) {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        uint32_t o[16];
+                        if (piece.b1 > piece.b0) tmem_ld16(lane_addr + GT_O + 64 * d + r0, o);
+                        tmem_wait_ld();
+                        if (left >= 16) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) dst[128 * d + i * D_V] = cvt(f[i] == 0.f ? 0.f : __uint_as_float(o[i]) * f[i]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (i < left) dst[128 * d + i * D_V] = cvt(f[i] == 0.f ? 0.f : __uint_as_float(o[i]) * f[i]);
                         }
                     }
-                }
+                };
+                if (whole) store(static_cast<uint16_t*>(p.out) + at, [](float v) { return out_bits<F16>(v); });
+                else store(p.o_part + at, [](float v) { return v; });
             }
             tc_fence_before();
             named_bar_sync(1, PG_SM_THREADS);                     // the factors have been read
@@ -406,66 +418,84 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
             // A warp per group of dims: a copy takes its warp about 130 cycles to issue, all of them from one warp 3900 cycles a block.
             const int rows = p.copy_rows, copies = 64 / rows;     // rows of a copy, copies of a block (and chunk): lane i sees to i and i + 32
             const int g = warp - LD0, c0 = 2 * g, c1 = g == 3 ? CHUNKS : c0 + 2;
-            int page[2], in[2];
-            unsigned v_lo, v_hi;                                  // rows that are there
-            uint32_t bytes;                                       // of a chunk
-            auto places = [&](int b) {                            // where block b's rows lie
+            // Where a block's rows lie, and which of them are there; looked up two blocks ahead and asked into L2 then: what waits for a
+            // free stage should not wait for HBM as well.
+            struct Places {
+                int page[2], in[2], q_row;
+                unsigned v_lo, v_hi;
+                uint32_t bytes;                                   // of a chunk
+                bool have, first;                                 // there is such a block; it is the first of its piece
+            };
+            int b = -1;
+            bool more = piece.next(p);
+            auto look_up = [&](Places& w) {                       // the next block in line
+                w.have = more;
+                if (!more) return;
+                if (b < 0) {
+                    while (piece.b1 == piece.b0) {
+                        if (!piece.next(p)) { w.have = more = false; return; }
+                    }
+                    b = piece.b0;
+                }
+                w.first = b == piece.b0;
+                w.q_row = piece.req * p.rows + row0;
                 unsigned long long valid = 0ull;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int i = lane + 32 * u, pos = b * 64 + i * rows;
-                    page[u] = -1;
-                    in[u] = 0;
+                    w.page[u] = -1;
+                    w.in[u] = 0;
                     if (i < copies && pos < piece.len) {
                         const int j = pos / p.page_block_size, e = ld_in(p.table + (int64_t)piece.req * p.table_stride + j);
                         if (e >= 0 && e < p.num_pages) {
-                            page[u] = e;
-                            in[u] = pos - j * p.page_block_size;
+                            w.page[u] = e;
+                            w.in[u] = pos - j * p.page_block_size;
                             const int k = min(piece.len - pos, rows);
                             valid |= (k == 64 ? ~0ull : (1ull << k) - 1ull) << (i * rows);
                         }
                     }
                 }
-                v_lo = __reduce_or_sync(0xffffffffu, (unsigned)valid);
-                v_hi = __reduce_or_sync(0xffffffffu, (unsigned)(valid >> 32));
-                bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, page[0] >= 0)) + __popc(__ballot_sync(0xffffffffu, page[1] >= 0))) * rows * 128u;
-            };
-            int b = 0;
-            bool first = true;
-            auto advance = [&](bool inside) {                     // to the next block
-                first = false;
-                if (inside && ++b < piece.b1) return true;
-                do {
-                    if (!piece.next(p)) return false;
-                } while (piece.b1 == piece.b0);
-                b = piece.b0;
-                first = true;
-                return true;
-            };
-            bool have = advance(false);
-            if (have) places(b);
-            for (; have && ok; ++it) {
-                const uint32_t st = it & 1, full = bar(GB_KFULL + 4 * st + g);
-                if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + 4 * st + g), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
-                if (ok && first && pieces > 0) ok = mbar_wait_lean(bar(GB_QFREE), (pieces - 1) & 1u, abort_addr, WP_QFREE);
-                if (!ok) break;
-                if (g == 0 && lane == 0) *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * st) = ((unsigned long long)v_hi << 32) | v_lo;
-                if (elect_one()) {
-                    mbar_arrive_expect_tx(full, (uint32_t)(c1 - c0) * (bytes + (first ? G_CHUNK : 0u)));
-                    if (first)
-                        for (int ch = c0; ch < c1; ++ch) tma_load_2d(base + GQ_OFF + ch * G_CHUNK, &q_map, ch * 64, piece.req * p.rows + row0, full);
+                w.v_lo = __reduce_or_sync(0xffffffffu, (unsigned)valid);
+                w.v_hi = __reduce_or_sync(0xffffffffu, (unsigned)(valid >> 32));
+                w.bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, w.page[0] >= 0)) + __popc(__ballot_sync(0xffffffffu, w.page[1] >= 0))) * rows * 128u;
+                if (++b == piece.b1) {
+                    more = piece.next(p);
+                    b = -1;
                 }
+            };
+            auto copy = [&](const Places& w, auto&& one) {        // one(copy's number, its page, its first row), under elect_one, with operands that are the same in all lanes
 #pragma unroll 1
-                for (int i = 0; i < copies; ++i) {                // (under elect_one, with operands that are the same in all lanes)
-                    const int e = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31), y = __shfl_sync(0xffffffffu, i < 32 ? in[0] : in[1], i & 31);
-                    if (e >= 0 && elect_one())
-                        for (int ch = c0; ch < c1; ++ch)
-                            tma_load_3d(base + GK_OFF + st * G_STAGE + ch * G_CHUNK + i * rows * 128, &k_map, ch * 64, y, e, full);
+                for (int i = 0; i < copies; ++i) {
+                    const int e = __shfl_sync(0xffffffffu, i < 32 ? w.page[0] : w.page[1], i & 31), y = __shfl_sync(0xffffffffu, i < 32 ? w.in[0] : w.in[1], i & 31);
+                    if (e >= 0 && elect_one()) one(i, e, y);
                 }
                 __syncwarp();
-                if (first) ++pieces;
-                have = advance(true);
-                if (have) places(b);                              // read while the stage is in use
+            };
+            Places w0, w1;
+            look_up(w0);
+            look_up(w1);
+            for (; w0.have && ok; ++it) {
+                const uint32_t st = it & 1, full = bar(GB_KFULL + 4 * st + g);
+                if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + 4 * st + g), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
+                if (ok && w0.first && pieces > 0) ok = mbar_wait_lean(bar(GB_QFREE), (pieces - 1) & 1u, abort_addr, WP_QFREE);
+                if (!ok) break;
+                if (g == 0 && lane == 0) *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * st) = ((unsigned long long)w0.v_hi << 32) | w0.v_lo;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(full, (uint32_t)(c1 - c0) * (w0.bytes + (w0.first ? G_CHUNK : 0u)));
+                    if (w0.first)
+                        for (int ch = c0; ch < c1; ++ch) tma_load_2d(base + GQ_OFF + ch * G_CHUNK, &q_map, ch * 64, w0.q_row, full);
+                }
+                const uint32_t dst = base + GK_OFF + st * G_STAGE;
+                copy(w0, [&](int i, int e, int y) {
+                    for (int ch = c0; ch < c1; ++ch) tma_load_3d(dst + ch * G_CHUNK + i * rows * 128, &k_map, ch * 64, y, e, full);
+                });
+                if (w0.first) ++pieces;
+                w0 = w1;
+                look_up(w1);
+                if (w1.have)
+                    copy(w1, [&](int, int e, int y) {
+                        for (int ch = c0; ch < c1; ++ch) tma_prefetch_3d(&k_map, ch * 64, y, e);
+                    });
             }
         } else {
             const int stage = (warp - LD0) >> 2, gw = (warp - LD0) & 3;
@@ -572,12 +602,17 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-#pragma unroll 1
-                        for (int ch = 2 * g; ch < (g == 3 ? CHUNKS : 2 * g + 2); ++ch) {
+                        const uint32_t qa = q_lo + ((2 * g * G_CHUNK) >> 4), ka = k_lo + ((st * G_STAGE + 2 * g * G_CHUNK) >> 4), d = tmem + GT_S + 64 * st;
+                        mma_f16(d, make_desc(qa, G_DESC_HI), make_desc(ka, G_DESC_HI), idesc, g != 0);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma_f16(tmem + GT_S + 64 * st, make_desc(q_lo + ((ch * G_CHUNK + k * 32) >> 4), G_DESC_HI),
-                                        make_desc(k_lo + ((st * G_STAGE + ch * G_CHUNK + k * 32) >> 4), G_DESC_HI), idesc, (ch | k) != 0);
+                        for (int k = 1; k < 8; ++k)
+                            mma_f16(d, make_desc(qa + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), G_DESC_HI),
+                                    make_desc(ka + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), G_DESC_HI), idesc, true);
+                        if (CHUNKS == 9 && g == 3) {
+#pragma unroll
+                            for (int k = 8; k < 12; ++k)
+                                mma_f16(d, make_desc(qa + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), G_DESC_HI),
+                                        make_desc(ka + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), G_DESC_HI), idesc, true);
                         }
                         if (g == 3) {
                             tc_commit(bar(GB_SREADY + st));
@@ -601,12 +636,13 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
-#pragma unroll 1
+                    const uint32_t va = v_lo + ((st * G_STAGE) >> 4);
+#pragma unroll
                     for (int d = 0; d < 4; ++d) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_f16(tmem + GT_O + 64 * d, make_desc(v_lo + ((st * G_STAGE + 2 * d * G_CHUNK + k * 2048) >> 4), G_DESC_HI),
-                                    make_desc(p_lo + ((k * 32) >> 4), G_DESC_HI), idesc, b != piece.b0 || k != 0);
+                            mma_f16(tmem + GT_O + 64 * d, make_desc(va + ((2 * d * G_CHUNK + k * 2048) >> 4), G_DESC_HI),
+                                    make_desc(p_lo + ((k * 32) >> 4), G_DESC_HI), idesc, k != 0 || b != piece.b0);
                         tc_commit(bar(GB_KFREE + 4 * st + d));
                     }
                     tc_commit(bar(GB_PVDONE));
@@ -630,16 +666,18 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
     if (warp == S_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// Four warps per query row of a request: join what its partitions left.  Requests within one partition are done.  Warp w sums records w,
-// w + 4, ..., four of them asked for at a time: the merge is a chain of latencies (one request of 131072 rows in 74 partitions: 64 us with one
-// warp per row and a record at a time).  The order of the sums is fixed.
+// Joins what a request's partitions left, a query row by one warp or, where requests lie in many partitions, by four: warp w sums records w,
+// w + W, ..., four of them asked for at a time.  It is a chain of latencies (one request of 131072 rows in 74 partitions: 64 us with one warp
+// per row and a record at a time, 11 with four), unless there are many rows: then more rows at a time hide it (64 requests of 128 heads
+// in 74 partitions: 25 us with four warps per row).  Requests within one partition are done.  The order of the sums is fixed.
 constexpr int PC_WARPS = 4, PC_AHEAD = 4;
-template <bool F16> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combine_kernel(const PagedParams p) {
-    __shared__ float4 sums[PC_WARPS - 1][D_V / 4];
+template <bool F16, int W> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combine_kernel(const PagedParams p) {
+    __shared__ float4 sums[W > 1 ? W - 1 : 1][D_V / 4];
     grid_dep_wait();
     grid_dep_launch();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t id = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0;
+    const int64_t id = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * PC_WARPS + (threadIdx.x >> 5);
+    if (id >= (int64_t)p.batch * p.rows) return;
     const int req = (int)(id / p.rows), row = (int)(id - (int64_t)req * p.rows);
     const uint2 span = ld_in(reinterpret_cast<const uint2*>(p.spans + req));
     const int c0 = (int)span.x, n = (int)span.y - c0 + 1;
@@ -649,8 +687,8 @@ template <bool F16> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combi
     auto load = [&](int s0) {
 #pragma unroll
         for (int u = 0; u < PC_AHEAD; ++u)
-            if (s0 + PC_WARPS * u < n) {
-                const float4* src = reinterpret_cast<const float4*>(p.o_part + record(s0 + PC_WARPS * u) * D_V) + lane;
+            if (s0 + W * u < n) {
+                const float4* src = reinterpret_cast<const float4*>(p.o_part + record(s0 + W * u) * D_V) + lane;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[u][i] = ld_in_once(src + 32 * i);
             }
@@ -674,11 +712,11 @@ template <bool F16> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combi
     float4 acc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = warp; s0 < n; s0 += PC_WARPS * PC_AHEAD) {
+    for (int s0 = warp; s0 < n; s0 += W * PC_AHEAD) {
         if (s0 > warp) load(s0);
 #pragma unroll
         for (int u = 0; u < PC_AHEAD; ++u) {
-            const int s = s0 + PC_WARPS * u;
+            const int s = s0 + W * u;
             if (s >= n) break;
             const float x = ld_in(p.lse_part + record(s)), w = x == NEG_BIG ? 0.f : exp2f(x - mx) * inv;
 #pragma unroll
@@ -687,18 +725,20 @@ template <bool F16> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combi
             }
         }
     }
-    if (warp > 0) {
+    if constexpr (W > 1) {
+        if (warp > 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[warp - 1][32 * i + lane] = acc[i];
-    }
-    __syncthreads();
-    if (warp > 0) return;
+            for (int i = 0; i < 4; ++i) sums[warp - 1][32 * i + lane] = acc[i];
+        }
+        __syncthreads();
+        if (warp > 0) return;
 #pragma unroll
-    for (int w = 0; w < PC_WARPS - 1; ++w) {
+        for (int w = 0; w < W - 1; ++w) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 x = sums[w][32 * i + lane];
-            acc[i].x += x.x; acc[i].y += x.y; acc[i].z += x.z; acc[i].w += x.w;
+            for (int i = 0; i < 4; ++i) {
+                const float4 x = sums[w][32 * i + lane];
+                acc[i].x += x.x; acc[i].y += x.y; acc[i].z += x.z; acc[i].w += x.w;
+            }
         }
     }
     if (lane == 0) p.lse[id] = lse;
@@ -760,7 +800,12 @@ int launch_attn_paged(PagedParams p, int layout, cudaStream_t stream) {
     launch_dependent(kernel, dim3(p.num_parts, (p.rows + PG_ROWS - 1) / PG_ROWS), dim3(paged_threads(layout)), G_SMEM, stream, p, q_map, k_map);
     if (int e = check_launch("attn_paged_kernel")) return e;
     if (p.num_parts == 1) return 0;                // every request is whole
-    launch_dependent(f16 ? paged_combine_kernel<true> : paged_combine_kernel<false>, dim3((unsigned)p.batch * (unsigned)p.rows), dim3(PC_WARPS * 32), 0, stream, p);
+    const unsigned rows = (unsigned)p.batch * (unsigned)p.rows;
+    const bool many = p.num_parts >= 4 * (int64_t)p.batch;
+    typedef void (*Combine)(const PagedParams);
+    const Combine combine = many ? (f16 ? paged_combine_kernel<true, PC_WARPS> : paged_combine_kernel<false, PC_WARPS>)
+                                 : (f16 ? paged_combine_kernel<true, 1> : paged_combine_kernel<false, 1>);
+    launch_dependent(combine, dim3(many ? rows : (rows + PC_WARPS - 1) / PC_WARPS), dim3(PC_WARPS * 32), 0, stream, p);
     return check_launch("paged_combine_kernel");
 }
 

@@ -186,6 +186,11 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tensor_map
                  ::"r"(dst), "l"(tensor_map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
+// Asks L2 for the box.
+__device__ __forceinline__ void tma_prefetch_3d(const void* tensor_map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(tensor_map), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 // Four rows of a 2-D tensor map (box one row high), the same columns of each, one after the other into shared memory.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tensor_map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"

@@ -52,6 +52,9 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
            ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16);
 }
 
+// a / b of numbers that are not negative, in 32 bits where they suffice (a 64-bit division takes a warp a hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) { return a <= 0xffffffffll ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
+
 // The 64 values of a rotated vector by eight lanes, eight values each: [8 l, 8 l + 8) where pairs are neighbours, else [4 l, 4 l + 4)
 // and the same 32 further.
 template <bool PAIRS> __device__ __forceinline__ uint4 ld_rot(const uint16_t* p, int l) {
@@ -84,12 +87,14 @@ template <int LAYOUT, bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) 
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const int64_t t = unit / p.parts;
+    const int64_t t = quotient(unit, p.parts);
     const int part = (int)(unit - t * p.parts), l = lane & 7;
     if (t >= p.num_tokens) return;
     float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+    // The values are asked for before the position, the table's entry and the slot are known: else a warp waits for memory two or three
+    // times in a row (8192 tokens of 128 heads 64.1 -> 53.9 us).
     const int64_t pos = p.positions != nullptr ? ld_index(p.positions, p.positions64, t) : 0;
-    if (p.positions != nullptr && (pos < 0 || pos >= p.num_positions)) return;       // a token without a position leaves nothing
+    const bool lost = p.positions != nullptr && (pos < 0 || pos >= p.num_positions);       // a token without a position leaves nothing
     if (part > 0) {
         const uint16_t* src = p.q_pe + t * p.q_pe_token;
         uint16_t* dst = p.q_out + t * p.q_out_token;
@@ -98,6 +103,7 @@ template <int LAYOUT, bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) 
 #pragma unroll
         for (int i = 0; i < KV_HEADS / 4; ++i)
             if (h0 + 4 * i < p.num_heads) v[i] = ld_rot<PAIRS>(src + (h0 + 4 * i) * p.q_pe_head, l);
+        if (lost) return;
         c = ld_in(reinterpret_cast<const float4*>(p.cos_sin + pos * 64) + l);
         s = ld_in(reinterpret_cast<const float4*>(p.cos_sin + pos * 64 + 32) + l);
 #pragma unroll
@@ -106,10 +112,6 @@ template <int LAYOUT, bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) 
         return;
     }
     const int64_t slot = ld_index(p.slots, p.slots64, t);
-    if (slot < 0 || slot >= p.capacity) return;
-    const int64_t page = slot / p.page_block_size;
-    const int in = (int)(slot - page * p.page_block_size);
-    uint8_t* base = p.cache + page * p.page_stride;
     const uint16_t* src = p.kv_c + t * p.kv_c_token;
     constexpr int NOPE = LAYOUT == SMLA_LAYOUT_MODEL1 ? 448 : 512;
     const bool mine = LAYOUT != SMLA_LAYOUT_MODEL1 || lane < 28;
@@ -120,8 +122,12 @@ template <int LAYOUT, bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) 
         a = ld_in_once(reinterpret_cast<const uint4*>(src + lane * (ROWS16 ? 8 : 16)));
         b = ld_in_once(reinterpret_cast<const uint4*>(src + (ROWS16 ? 256 + lane * 8 : lane * 16 + 8)));
     }
+    if (lane < 8) r = ld_rot<PAIRS>(p.k_pe + t * p.k_pe_token, l);
+    if (lost || slot < 0 || slot >= p.capacity) return;
+    const int64_t page = quotient(slot, p.page_block_size);
+    const int in = (int)(slot - page * p.page_block_size);
+    uint8_t* base = p.cache + page * p.page_stride;
     if (lane < 8) {
-        r = ld_rot<PAIRS>(p.k_pe + t * p.k_pe_token, l);
         if (p.positions != nullptr) {
             c = ld_in(reinterpret_cast<const float4*>(p.cos_sin + pos * 64) + l);
             s = ld_in(reinterpret_cast<const float4*>(p.cos_sin + pos * 64 + 32) + l);
@@ -194,11 +200,10 @@ template <bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) append_index
     grid_dep_launch();
     const int lane = threadIdx.x & 31, l = lane & 15;
     const int64_t unit = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const int64_t t = unit / p.parts;
+    const int64_t t = quotient(unit, p.parts);
     const int part = (int)(unit - t * p.parts);
     if (t >= p.num_tokens) return;
     const int64_t pos = p.positions != nullptr ? ld_index(p.positions, p.positions64, t) : 0;
-    if (p.positions != nullptr && (pos < 0 || pos >= p.num_positions)) return;
     constexpr int N = IX_HEADS / 2;
     const int rows = part == 0 ? 1 : min(p.num_heads - (part - 1) * IX_HEADS, IX_HEADS);
     const int64_t row0 = part == 0 ? t : t * p.num_heads + (part - 1) * IX_HEADS;
@@ -209,6 +214,9 @@ template <bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) append_index
         v[i] = make_uint4(0, 0, 0, 0);
         if (2 * i + (lane >> 4) < rows) v[i] = ld_in_once(reinterpret_cast<const uint4*>(src + (2 * i + (lane >> 4)) * 128 + l * 8));
     }
+    int64_t slot = 0;
+    if (part == 0) slot = ld_index(p.slots, p.slots64, t);
+    if (p.positions != nullptr && (pos < 0 || pos >= p.num_positions)) return;
     // the rotated half of the row lies in eight neighbouring lanes
     const bool turns = p.positions != nullptr && (l >> 3) == (p.rope_offset >> 6);
     float c[8], s[8];
@@ -229,8 +237,6 @@ template <bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) append_index
             }
         }
     }
-    int64_t slot = 0;
-    if (part == 0) slot = ld_index(p.slots, p.slots64, t);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (2 * i >= rows) break;
@@ -262,10 +268,22 @@ template <bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) append_index
         for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float scale = __fdiv_rn(fmaxf(amax, 1e-4f), 448.f);
+        const float scale = __fdiv_rn(fmaxf(amax, 1e-4f), 448.f), inv = __fdiv_rn(1.f, scale);
+        // x / scale, rounded to fp32 and then to e4m3.  x inv lies within two steps of fp32 of it, so both give the same e4m3 value unless a
+        // border of e4m3's rounding (the middle of two of its values: 20 bits of the fp32 mantissa say 1000...) is as near; only then,
+        // once in some 30000 values, and below e4m3's normal range, the warp divides.  (A division takes some ten instructions.)
+        float z[8];
+        bool near = false;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fdiv_rn(x[j], scale);
-        const uint2 y = make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
+        for (int j = 0; j < 8; ++j) {
+            z[j] = x[j] * inv;
+            near |= ((__float_as_uint(z[j]) - 0x7fffdu) & 0xfffffu) <= 6u || fabsf(z[j]) < 0x1p-6f;
+        }
+        if (near) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = __fdiv_rn(x[j], scale);
+        }
+        const uint2 y = make_uint2(e4m3x4(z[0], z[1], z[2], z[3]), e4m3x4(z[4], z[5], z[6], z[7]));
         const int r = 2 * i + (lane >> 4);
         if (r >= rows) continue;
         if (part == 0) {

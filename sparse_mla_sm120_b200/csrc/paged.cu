@@ -30,8 +30,9 @@ using namespace ptx;
 using namespace attn;
 
 constexpr int PG_ROWS = 64;                       // query rows of a CTA
-constexpr int PG_START = 2;                       // blocks' worth of time that a request takes before its first row
-constexpr int PG_LEAST = 2;                       // blocks of rows that a partition should be worth
+// Blocks' worth of time that a request takes before its first row; no partition is shorter.  (Partitions of four blocks at least, for less
+// to merge where SMs are idle: one request of 1000 rows, 16 heads, 15.2 us instead of 13.3.)
+constexpr int PG_START = 2;
 constexpr int PG_SM_WARPS = 8, PG_SM_THREADS = PG_SM_WARPS * 32;
 __host__ __device__ constexpr bool packed_rows(int layout) { return layout == SMLA_LAYOUT_V32 || layout == SMLA_LAYOUT_MODEL1; }
 __host__ __device__ constexpr int load_warps(int layout) { return packed_rows(layout) ? 8 : 4; }
@@ -78,7 +79,7 @@ __device__ __forceinline__ int paged_blocks(int len) { return (int)(((unsigned)l
 __host__ __device__ __forceinline__ long long paged_share(long long total, int parts) {
     // (a 64-bit division takes hundreds of cycles)
     const long long u = total + parts <= 0xffffffffll ? (long long)((unsigned)(total + parts - 1) / (unsigned)parts) : (total + parts - 1) / parts;
-    return u > PG_START + PG_LEAST ? u : PG_START + PG_LEAST;
+    return u > PG_START ? u : PG_START;
 }
 
 // The pieces of a partition, one after the other: request, its rows, and which of its blocks are the partition's.
@@ -757,7 +758,7 @@ int paged_parts(int batch, int rows, int pages_per_request, int page_block_size,
     if (sms < 1) return 0;
     const int groups = (rows + PG_ROWS - 1) / PG_ROWS, most = sms / groups > 0 ? sms / groups : 1;
     const long long blocks = ((long long)pages_per_request * page_block_size + 63) / 64;
-    const long long worth = (batch * (blocks + PG_START) + PG_START + PG_LEAST - 1) / (PG_START + PG_LEAST);
+    const long long worth = (batch * (blocks + PG_START) + PG_START - 1) / PG_START;
     return worth < most ? (int)(worth > 0 ? worth : 1) : most;
 }
 

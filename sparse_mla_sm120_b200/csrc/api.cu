@@ -1,5 +1,6 @@
 // extern "C" entry points of libsmla_b200.so: argument checks, error strings, dispatch.
 // No torch types, no allocation, no host synchronisation.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 
@@ -68,6 +69,10 @@ const char* smla_status_string(int code) {
         case 61: return "paged attention rows stored"; case 62: return "paged attention rows free"; case 63: return "paged attention s_ready";
         case 64: return "paged attention p_ready"; case 65: return "paged attention pv_done"; case 66: return "paged attention q_free";
         case 67: return "paged attention s_free";
+        case 91: return "paged attention pair k_full"; case 92: return "paged attention pair k_peer"; case 93: return "paged attention pair k_free";
+        case 94: return "paged attention pair v_full"; case 95: return "paged attention pair v_peer"; case 96: return "paged attention pair v_free";
+        case 97: return "paged attention pair s_ready"; case 98: return "paged attention pair s_free"; case 99: return "paged attention pair p_ready";
+        case 100: return "paged attention pair pv_done"; case 101: return "paged attention pair q_free";
         case 51: return "attention tile k_full"; case 52: return "attention tile rope_full"; case 53: return "attention tile k_free";
         case 54: return "attention tile s_ready"; case 55: return "attention tile s_free"; case 56: return "attention tile scales";
         case 57: return "attention tile p_ready"; case 58: return "attention tile pv_done"; case 59: return "attention tile q_ready";
@@ -543,7 +548,9 @@ static size_t paged_spans_at(int parts, size_t rows) {
 
 size_t smla_paged_scratch_bytes(int batch, int query_len, int num_heads, int pages_per_request, int page_block_size, int num_parts) {
     if (paged_shape("smla_paged_scratch_bytes", batch, query_len, num_heads, pages_per_request, page_block_size, num_parts)) return 0;
-    const int parts = paged_parts(batch, query_len * num_heads, pages_per_request, page_block_size, num_parts);
+    // (of either kernel: the layout decides, and that is not asked here)
+    const int rows = query_len * num_heads, parts = std::max(paged_parts(batch, rows, pages_per_request, page_block_size, num_parts, false),
+                                                              paged_parts(batch, rows, pages_per_request, page_block_size, num_parts, true));
     return parts < 1 ? 0 : paged_spans_at(parts, (size_t)query_len * num_heads) + (size_t)batch * sizeof(int2);
 }
 
@@ -560,7 +567,7 @@ int smla_paged_decode(const void* q, const void* cache, int layout, int64_t num_
     if (!aligned16(q) || !aligned16(out) || !aligned16(scratch)) return set_error(SMLA_E_ALIGN, "%s: q, out and scratch must be 16-byte aligned", fn);
     PagedParams p{};
     p.rows = query_len * num_heads;
-    p.num_parts = paged_parts(batch, p.rows, pages_per_request, page_block_size, num_parts);
+    p.num_parts = paged_parts(batch, p.rows, pages_per_request, page_block_size, num_parts, paged_on_pairs(p.rows, layout));
     if (p.num_parts < 1) return SMLA_E_DEVICE;
     const size_t need = paged_spans_at(p.num_parts, p.rows) + (size_t)batch * sizeof(int2);
     if ((int64_t)batch * p.rows > 0x7fffffff) return set_error(SMLA_E_SHAPE, "%s: batch=%d of %d query rows", fn, batch, p.rows);

@@ -228,7 +228,8 @@ int launch_attn_exact(const AttnParams& p, cudaStream_t stream);   // MODEL1 lay
 bool attn_pair_takes(const AttnParams& p);   // alignment of the caches that the tensor-core kernel's bulk copies need
 int launch_append_kv(AppendKvParams p, int layout, bool pairs, cudaStream_t stream);
 int launch_append_index(AppendIndexParams p, bool pairs, cudaStream_t stream);
-int paged_parts(int batch, int rows, int pages_per_request, int page_block_size, int num_parts);   // partitions of a call, 0: an error is set
+bool paged_on_pairs(int rows, int layout);   // attn_paged_pair_kernel takes the call
+int paged_parts(int batch, int rows, int pages_per_request, int page_block_size, int num_parts, bool pairs);   // partitions of a call, 0: an error is set
 int launch_attn_paged(PagedParams p, int layout, cudaStream_t stream);
 int launch_pack_kv(const __nv_bfloat16* kv, uint8_t* packed, int64_t num_rows, cudaStream_t stream);
 int launch_mqa_logits_scalar(const uint8_t* q, const uint8_t* k, const float* k_scale, const float* weights,

@@ -18,9 +18,8 @@
 // is exact in bf16; four for even blocks, four for odd ones).  A stage is filled and freed in four groups of 128 dims, so that scores
 // begin when a quarter of the rows is there, and the next rows come when P.V is through with a quarter.
 // Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
-#include "attn_common.cuh"
+#include "paged_common.cuh"
 #include "rows_map.cuh"
-#include "sm100_ptx.cuh"
 
 namespace smla {
 
@@ -30,22 +29,14 @@ using namespace ptx;
 using namespace attn;
 
 constexpr int PG_ROWS = 64;                       // query rows of a CTA
-// Blocks' worth of time that a request takes before its first row; no partition is shorter.  (Partitions of four blocks at least, for less
-// to merge where SMs are idle: one request of 1000 rows, 16 heads, 15.2 us instead of 13.3.)
-constexpr int PG_START = 2;
 constexpr int PG_SM_WARPS = 8, PG_SM_THREADS = PG_SM_WARPS * 32;
 __host__ __device__ constexpr bool packed_rows(int layout) { return layout == SMLA_LAYOUT_V32 || layout == SMLA_LAYOUT_MODEL1; }
 __host__ __device__ constexpr int load_warps(int layout) { return packed_rows(layout) ? 8 : 4; }
 __host__ __device__ constexpr int paged_threads(int layout) { return packed_rows(layout) ? 640 : 448; }       // (packed: whole groups of four warps)
-// The running maximum of a row lags by at most 2^PG_TAU: weights are floating point, so that costs no precision (fp16 weights reach
-// 2^8 and fall to zero 2^-24 below a maximum that does not lag), and the accumulator is rescaled a few times per request.
-constexpr float PG_TAU = 8.0f;
-
 // registers of the packed layouts' instances, which the loading warps take from the others
 constexpr int PG_REGS_LAUNCH = 96, PG_REGS_SOFTMAX = 88, PG_REGS_LOAD = 120, PG_REGS_MMA = 48;
 static_assert(PG_SM_WARPS * 32 * PG_REGS_SOFTMAX + 8 * 32 * PG_REGS_LOAD + 4 * 32 * PG_REGS_MMA <= 640 * PG_REGS_LAUNCH, "register budgets exceed what the CTA owns");
 
-constexpr uint32_t G_CHUNK = 64 * 128;            // 64 dims of 64 rows
 constexpr uint32_t G_STAGE = 9 * G_CHUNK;
 constexpr uint32_t GQ_OFF = 0;
 constexpr uint32_t GK_OFF = GQ_OFF + G_STAGE;
@@ -67,67 +58,6 @@ constexpr uint32_t GT_O = 0, GT_S = 256;          // tensor memory: dims block b
 constexpr uint32_t G_DESC_HI = desc_hi(1024, (uint32_t)SWIZZLE_128B);
 
 enum { WP_KFULL = 61, WP_KFREE = 62, WP_SREADY = 63, WP_PREADY = 64, WP_PVDONE = 65, WP_QFREE = 66, WP_SFREE = 67 };
-
-__device__ __forceinline__ uint32_t gswz(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
-
-__device__ __forceinline__ int paged_length(const PagedParams& p, int req) {
-    const long long most = (long long)p.pages_per_request * p.page_block_size;
-    const int n = max(ld_in(p.lengths + req), 0);
-    return n < most ? n : (int)most;
-}
-__device__ __forceinline__ int paged_blocks(int len) { return (int)(((unsigned)len + 63u) >> 6); }
-__host__ __device__ __forceinline__ long long paged_share(long long total, int parts) {
-    // (a 64-bit division takes hundreds of cycles)
-    const long long u = total + parts <= 0xffffffffll ? (long long)((unsigned)(total + parts - 1) / (unsigned)parts) : (total + parts - 1) / parts;
-    return u > PG_START ? u : PG_START;
-}
-
-// The pieces of a partition, one after the other: request, its rows, and which of its blocks are the partition's.
-struct Pieces {
-    long long lo, hi, start;       // the partition's part of the line, and where the request begins on it
-    int req, len, nb, b0, b1;
-    bool begun;
-    __device__ __forceinline__ Pieces(long long lo_, long long hi_, int req_, long long start_) : lo(lo_), hi(hi_), start(start_), req(req_), begun(false) {}
-    __device__ __forceinline__ bool next(const PagedParams& p) {
-        while (true) {
-            if (begun) { start += nb + PG_START; ++req; }
-            begun = true;
-            if (req >= p.batch || start >= hi) return false;
-            len = paged_length(p, req);
-            nb = paged_blocks(len);
-            const long long first = start + PG_START;
-            b0 = (int)max(lo - first, 0ll);
-            b1 = (int)min(hi - first, (long long)nb);
-            if (b1 > b0) return true;
-            if (nb == 0 && first - 1 >= lo && first - 1 < hi) { b0 = b1 = 0; return true; }      // a request without rows: whoever holds its last unit
-        }
-    }
-    __device__ __forceinline__ bool whole() const { return b0 == 0 && b1 == nb; }
-};
-
-// log2(2^a + 2^b)
-__device__ __forceinline__ float log2_add(float a, float b) {
-    const float hi = fmaxf(a, b), lo = fminf(a, b);
-    return (hi == INFINITY || hi == -INFINITY) ? hi : hi + log2f(1.f + exp2f(lo - hi));
-}
-// LSE of a row with a sink: `lse` is NEG_BIG where the row sees nothing.
-__device__ __forceinline__ float with_sink(float lse, float sink2) {
-    if (lse != NEG_BIG) return log2_add(lse, sink2);
-    return sink2 == -INFINITY ? NEG_BIG : sink2;
-}
-
-template <bool F16> __device__ __forceinline__ uint32_t pack_weights(float a, float b) {
-    if (F16) {
-        const __half2 r = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <bool F16> __device__ __forceinline__ uint16_t out_bits(float v) {
-    if (F16) return __half_as_ushort(__float2half_rn(v));
-    return __bfloat16_as_ushort(__float2bfloat16_rn(v));
-}
 
 // Sixteen e4m3 values times their scale as bf16 (exact for powers of two; no number stays none).
 __device__ __forceinline__ void dequant16(uint4 v, float scale, uint32_t (&d)[8]) {
@@ -180,41 +110,7 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
     grid_dep_wait();
     grid_dep_launch();
 
-    // ---- the partition's part of the line: every thread sums the requests of its share, the block scans the sums
-    long long* scan = reinterpret_cast<long long*>(sm + GW_OFF);
-    const int per = (p.batch + (int)blockDim.x - 1) / (int)blockDim.x;
-    const int r_lo = min(tid * per, p.batch), r_hi = min(r_lo + per, p.batch);
-    long long sum = 0;
-    for (int r = r_lo; r < r_hi; ++r) sum += paged_blocks(paged_length(p, r)) + PG_START;
-    long long incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    if (lane == 31) scan[warp] = incl;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    long long before = incl - sum, total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) before += scan[w];
-        total += scan[w];
-    }
-    const long long share = paged_share(total, p.num_parts), lo = min(part * share, total), hi = min(lo + share, total);
-    if (before <= lo && lo < before + sum) {
-        int r = r_lo;
-        for (; r < r_hi - 1; ++r) {
-            const int w = paged_blocks(paged_length(p, r)) + PG_START;
-            if (lo < before + w) break;
-            before += w;
-        }
-        scan[20] = before;
-        *reinterpret_cast<int*>(scan + 21) = r;
-    }
-    __syncthreads();
-    Pieces piece(lo, hi, lo < hi ? *reinterpret_cast<int*>(scan + 21) : p.batch, lo < hi ? scan[20] : 0);
+    Pieces<64> piece = partition_of<64>(p, part, reinterpret_cast<long long*>(sm + GW_OFF), WARPS);
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + GMISC_OFF);
     if (PACKED) {
         if (warp < PG_SM_WARPS) setmaxnreg_dec<PG_REGS_SOFTMAX>();
@@ -238,14 +134,9 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
         while (!stop && piece.next(p)) {
             const bool whole = piece.whole();
             if (row0 == 0 && tid == 0 && piece.b0 == 0) {
-                const long long end = piece.start + PG_START + piece.nb - 1;
-                const int last = whole ? part : (int)(end <= 0xffffffffll && share <= end ? (unsigned)end / (unsigned)share : end / share);
-                p.spans[piece.req] = make_int2(part, last);
+                piece.write_span(p, part);
             }
-            // rows that query rows see: all of the request's, or up to the query's own
-            const int hidden = p.causal ? p.query_len - 1 : 0;
-            auto sees = [&](int r) { return p.causal ? min(max(piece.len - hidden + min(row0 + r, p.rows - 1) / p.num_heads, 0), piece.len) : piece.len; };
-            const int see_a = sees(ra), see_b = sees(rb), see_least = sees(0);
+            const int see_a = paged_sees(p, piece.len, row0 + ra), see_b = paged_sees(p, piece.len, row0 + rb), see_least = paged_sees(p, piece.len, row0);
             float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
             for (int b = piece.b0; b < piece.b1; ++b, ++it) {
                 const uint32_t st = it & 1;
@@ -752,12 +643,15 @@ template <bool F16, int W> __global__ void __launch_bounds__(PC_WARPS * 32) page
 
 }  // namespace
 
-int paged_parts(int batch, int rows, int pages_per_request, int page_block_size, int num_parts) {
+bool paged_on_pairs(int rows, int layout) { return rows > PG_ROWS && !packed_rows(layout); }
+
+int paged_parts(int batch, int rows, int pages_per_request, int page_block_size, int num_parts, bool pairs) {
     if (num_parts > 0) return num_parts;
     const int sms = smla_num_sms();
     if (sms < 1) return 0;
-    const int groups = (rows + PG_ROWS - 1) / PG_ROWS, most = sms / groups > 0 ? sms / groups : 1;
-    const long long blocks = ((long long)pages_per_request * page_block_size + 63) / 64;
+    const int unit = pairs ? 2 * PG_ROWS : PG_ROWS;               // query rows, and cache rows of a block
+    const int groups = (rows + unit - 1) / unit, room = pairs ? sms / 2 : sms, most = room / groups > 0 ? room / groups : 1;
+    const long long blocks = ((long long)pages_per_request * page_block_size + unit - 1) / unit;
     const long long worth = (batch * (blocks + PG_START) + PG_START - 1) / PG_START;
     return worth < most ? (int)(worth > 0 ? worth : 1) : most;
 }
@@ -794,12 +688,18 @@ int launch_attn_paged(PagedParams p, int layout, cudaStream_t stream) {
         const uint32_t k_box[3] = {64, (uint32_t)p.copy_rows, 1};
         if (int e = encode_map(&k_map, type, 3, p.cache, k_dims, k_strides, k_box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
     }
+    const bool pairs = paged_on_pairs(p.rows, layout);
+    if (pairs) {
+        if (int e = launch_attn_paged_pair(p, f16, q_map, k_map, stream)) return e;
+    }
     const Kernel kernel = layout == SMLA_LAYOUT_V32      ? attn_paged_kernel<SMLA_LAYOUT_V32>
                           : layout == SMLA_LAYOUT_MODEL1 ? attn_paged_kernel<SMLA_LAYOUT_MODEL1>
                           : layout == SMLA_LAYOUT_BF16   ? attn_paged_kernel<SMLA_LAYOUT_BF16>
                                                          : attn_paged_kernel<SMLA_LAYOUT_F16>;
-    launch_dependent(kernel, dim3(p.num_parts, (p.rows + PG_ROWS - 1) / PG_ROWS), dim3(paged_threads(layout)), G_SMEM, stream, p, q_map, k_map);
-    if (int e = check_launch("attn_paged_kernel")) return e;
+    if (!pairs) {
+        launch_dependent(kernel, dim3(p.num_parts, (p.rows + PG_ROWS - 1) / PG_ROWS), dim3(paged_threads(layout)), G_SMEM, stream, p, q_map, k_map);
+        if (int e = check_launch("attn_paged_kernel")) return e;
+    }
     if (p.num_parts == 1) return 0;                // every request is whole
     const unsigned rows = (unsigned)p.batch * (unsigned)p.rows;
     const bool many = p.num_parts >= 4 * (int64_t)p.batch;

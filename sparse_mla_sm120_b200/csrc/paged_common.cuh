@@ -1,0 +1,141 @@
+// What the kernels of attention over a block table share (paged.cu, paged_pair.cu): how requests' rows are cut into partitions, masks of
+// the LSE, 16-bit forms.
+#pragma once
+
+#include "attn_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace smla {
+
+namespace {
+
+using namespace ptx;
+using namespace attn;
+
+// Blocks' worth of time that a request takes before its first row; no partition is shorter.  (Partitions of four blocks at least, for less
+// to merge where SMs are idle: one request of 1000 rows, 16 heads, 15.2 us instead of 13.3.)
+constexpr int PG_START = 2;
+// The running maximum of a row lags by at most 2^PG_TAU: weights are floating point, so that costs no precision (fp16 weights reach
+// 2^8 and fall to zero 2^-24 below a maximum that does not lag), and the accumulator is rescaled a few times per request.
+constexpr float PG_TAU = 8.0f;
+constexpr uint32_t G_CHUNK = 64 * 128;            // 64 dims of 64 rows, 128B swizzle
+
+__device__ __forceinline__ uint32_t gswz(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
+
+__device__ __forceinline__ int paged_length(const PagedParams& p, int req) {
+    const long long most = (long long)p.pages_per_request * p.page_block_size;
+    const int n = max(ld_in(p.lengths + req), 0);
+    return n < most ? n : (int)most;
+}
+template <int ROWS> __device__ __forceinline__ int paged_blocks(int len) { return (int)(((unsigned)len + (ROWS - 1u)) / (unsigned)ROWS); }
+__device__ __forceinline__ long long paged_share(long long total, int parts) {
+    // (a 64-bit division takes hundreds of cycles)
+    const long long u = total + parts <= 0xffffffffll ? (long long)((unsigned)(total + parts - 1) / (unsigned)parts) : (total + parts - 1) / parts;
+    return u > PG_START ? u : PG_START;
+}
+
+// The pieces of a partition, one after the other: request, its rows, and which of its blocks of ROWS rows are the partition's.
+template <int ROWS> struct Pieces {
+    long long lo, hi, start, share;       // the partition's part of the line, where the request begins on it, the length of a part
+    int req, len, nb, b0, b1;
+    bool begun;
+    __device__ __forceinline__ bool next(const PagedParams& p) {
+        while (true) {
+            if (begun) { start += nb + PG_START; ++req; }
+            begun = true;
+            if (req >= p.batch || start >= hi) return false;
+            len = paged_length(p, req);
+            nb = paged_blocks<ROWS>(len);
+            const long long first = start + PG_START;
+            b0 = (int)max(lo - first, 0ll);
+            b1 = (int)min(hi - first, (long long)nb);
+            if (b1 > b0) return true;
+            if (nb == 0 && first - 1 >= lo && first - 1 < hi) { b0 = b1 = 0; return true; }      // a request without rows: whoever holds its last unit
+        }
+    }
+    __device__ __forceinline__ bool whole() const { return b0 == 0 && b1 == nb; }
+    // What the merge needs to know, written by the partition that has the request's first block.
+    __device__ __forceinline__ void write_span(const PagedParams& p, int part) const {
+        const long long end = start + PG_START + nb - 1;
+        const int last = whole() ? part : (int)(end <= 0xffffffffll && share <= end ? (unsigned)end / (unsigned)share : end / share);
+        p.spans[req] = make_int2(part, last);
+    }
+};
+
+// The partition's part of the line: every thread sums the requests of its share, the block (of `warps` warps) scans the sums.  scan: 22
+// words of shared memory.  Synchronises the block, tensor memory's address included.
+template <int ROWS> __device__ __forceinline__ Pieces<ROWS> partition_of(const PagedParams& p, int part, long long* scan, int warps) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int per = (p.batch + (int)blockDim.x - 1) / (int)blockDim.x;
+    const int r_lo = min(tid * per, p.batch), r_hi = min(r_lo + per, p.batch);
+    long long sum = 0;
+    for (int r = r_lo; r < r_hi; ++r) sum += paged_blocks<ROWS>(paged_length(p, r)) + PG_START;
+    long long incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    long long before = incl - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+    }
+    const long long share = paged_share(total, p.num_parts), lo = min(part * share, total), hi = min(lo + share, total);
+    if (before <= lo && lo < before + sum) {
+        int r = r_lo;
+        for (; r < r_hi - 1; ++r) {
+            const int w = paged_blocks<ROWS>(paged_length(p, r)) + PG_START;
+            if (lo < before + w) break;
+            before += w;
+        }
+        scan[20] = before;
+        *reinterpret_cast<int*>(scan + 21) = r;
+    }
+    __syncthreads();
+    Pieces<ROWS> piece;
+    piece.lo = lo; piece.hi = hi; piece.share = share;
+    piece.start = lo < hi ? scan[20] : 0;
+    piece.req = lo < hi ? *reinterpret_cast<int*>(scan + 21) : p.batch;
+    piece.begun = false;
+    return piece;
+}
+
+// Rows of the request that a query row sees: all, or up to the query's own.
+__device__ __forceinline__ int paged_sees(const PagedParams& p, int len, int row) {
+    if (!p.causal) return len;
+    return min(max(len - (p.query_len - 1) + min(row, p.rows - 1) / p.num_heads, 0), len);
+}
+
+// log2(2^a + 2^b)
+__device__ __forceinline__ float log2_add(float a, float b) {
+    const float hi = fmaxf(a, b), lo = fminf(a, b);
+    return (hi == INFINITY || hi == -INFINITY) ? hi : hi + log2f(1.f + exp2f(lo - hi));
+}
+// LSE of a row with a sink: `lse` is NEG_BIG where the row sees nothing.
+__device__ __forceinline__ float with_sink(float lse, float sink2) {
+    if (lse != NEG_BIG) return log2_add(lse, sink2);
+    return sink2 == -INFINITY ? NEG_BIG : sink2;
+}
+
+template <bool F16> __device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+    if (F16) {
+        const __half2 r = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <bool F16> __device__ __forceinline__ uint16_t out_bits(float v) {
+    if (F16) return __half_as_ushort(__float2half_rn(v));
+    return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+}  // namespace
+
+}  // namespace smla

@@ -1,0 +1,512 @@
+// Attention over a block table of more than 64 query rows per request, 16-bit rows: attn_paged_kernel's work on a pair of SMs
+// (tcgen05.mma.cta_group::2), 128 query rows and blocks of 128 cache rows.
+//
+// The formulas, the line of blocks that partitions cut, records and merge are those of paged.cu.  A cluster of two CTAs has 128 query rows, 64
+// each, and every MMA runs over the pair with M = 128:
+//   * S = Q . K^T: A = the CTA's queries, B = the 64 of the block's 128 rows that it has brought in (9 chunks of 64 dims, K-major);
+//     lanes 0-63 of a CTA's tensor memory get its query rows against rows 0-63 of the block, lanes 64-127 against rows 64-127;
+//   * O += P . V: A = the CTA's weights [64 x 128 rows], B = dims [256 r, +256) of all 128 rows in CTA r (MN-major), N = 256 in two
+//     products; lanes 0-63 get dims 0-255, lanes 64-127 dims 256-511: 256 columns of tensor memory.
+// Why a pair: operands of 64 rows keep the tensor core waiting for shared memory (M = N = 64: 40.6 cycles of the 16 that the arithmetic
+// takes; measured over 36 products in a row).  Over the pair M = N = 128 takes 41.8 for four times the products of one of the
+// CTAs' 64 x 64, M = 128 and N = 256 70: 2630 cycles per 128 x 128 where two CTAs of paged.cu take 4600.
+// What it costs: V comes in beside K (64 KB next to 72 KB per CTA and block, from L2), since a CTA has other dims of other rows in V than
+// in K, and the two fill shared memory: one stage of each, freed and filled again in parts while the products of the others run.
+//
+// Warps: 0-7 softmax and epilogue (thread = one query row x 32 rows of a block), 8-11 bring in K (two or three chunks each) and the queries, 12-15
+// V (64 rows x 128 dims each), 16 issues the score products, 17 those with V: both in the even CTA, in the odd one they pass on that its
+// K and V have landed.  Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
+#include "paged_common.cuh"
+#include "rows_map.cuh"
+
+namespace smla {
+
+namespace {
+
+constexpr int PP_TILE = 128;                      // cache rows of a block, and query rows of a pair
+constexpr int PP_SM_WARPS = 8, PP_K0 = 8, PP_V0 = 12, PP_S_WARP = 16, PP_WARPS = 18, PP_THREADS = PP_WARPS * 32;
+constexpr int PP_CHUNKS = 9;
+
+constexpr uint32_t PPQ_OFF = 0;
+constexpr uint32_t PPK_OFF = PPQ_OFF + PP_CHUNKS * G_CHUNK;
+constexpr uint32_t PPV_OFF = PPK_OFF + PP_CHUNKS * G_CHUNK;   // [2 halves of the block's rows][4 chunks of 64 dims]
+constexpr uint32_t PPP_OFF = PPV_OFF + 8 * G_CHUNK;           // weights: [2 halves of the block's rows][64 query rows][64]
+constexpr uint32_t PPX_OFF = PPP_OFF + 2 * G_CHUNK;           // [4][64] fp32: maxima, then sums, of the four threads of a query row
+constexpr uint32_t PPW_OFF = PPX_OFF + 4 * 64 * 4;            // schedule, 22 words
+constexpr uint32_t PPY_OFF = PPW_OFF + 22 * 8;                // which of a block's rows are there, [4 blocks] 128 bits
+constexpr uint32_t PPB_OFF = PPY_OFF + 4 * 16;
+// Barriers; those with a P collect arrivals of both CTAs and are used in the even one only.
+constexpr int PB_KFULL = 0, PB_KPEERP = 4, PB_KFREE = 8, PB_VFULL = 12, PB_VPEERP = 14, PB_VFREE = 16, PB_SREADY = 18, PB_SFREEP = 20, PB_PREADYP = 22,
+              PB_PVDONE = 23, PB_QFREE = 24, PB_N = 25;
+constexpr uint32_t PPMISC_OFF = PPB_OFF + PB_N * 8;
+constexpr uint32_t PP_SMEM = (PPMISC_OFF + 8 + 15) / 16 * 16 + 1024;
+static_assert(PP_SMEM <= 227 * 1024, "shared memory budget");
+static_assert(PPY_OFF % 16 == 0 && PPB_OFF % 8 == 0 && PPMISC_OFF % 8 == 0, "alignment");
+
+constexpr uint32_t PPT_O = 0, PPT_S = 256;        // tensor memory: O 2 x 128 columns, two score buffers of 64
+constexpr uint32_t PP_DESC_HI = desc_hi(1024, (uint32_t)SWIZZLE_128B);
+
+enum { WQ_KFULL = 91, WQ_KPEER = 92, WQ_KFREE = 93, WQ_VFULL = 94, WQ_VPEER = 95, WQ_VFREE = 96, WQ_SREADY = 97, WQ_SFREE = 98, WQ_PREADY = 99, WQ_PVDONE = 100,
+       WQ_QFREE = 101 };
+
+// The block's rows that are there and the pages of their copies: lane i sees to copies i, i + 32, i + 64 and i + 96 of `rows` rows each.
+struct BlockPlaces {
+    int page[4], in[4], q_row;
+    uint32_t valid[4];                            // the same in all lanes
+    bool have, first;                             // there is such a block; it is the first of its piece
+};
+
+// Walks a partition's blocks.
+struct BlockWalk {
+    Pieces<PP_TILE> piece;
+    int b;
+    bool more;
+    __device__ __forceinline__ BlockWalk(const PagedParams& p, const Pieces<PP_TILE>& first) : piece(first), b(-1) { more = piece.next(p); }
+    __device__ __forceinline__ void look_up(const PagedParams& p, int row0, BlockPlaces& w) {
+        w.have = more;
+        if (!more) return;
+        if (b < 0) {
+            while (piece.b1 == piece.b0) {
+                if (!piece.next(p)) { w.have = more = false; return; }
+            }
+            b = piece.b0;
+        }
+        w.first = b == piece.b0;
+        w.q_row = piece.req * p.rows + row0;
+        const int lane = threadIdx.x & 31, rows = p.copy_rows, copies = PP_TILE / rows;
+        uint32_t mine[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = lane + 32 * u;
+            w.page[u] = -1;
+            w.in[u] = 0;
+            if (i >= copies) continue;
+            const int pos = b * PP_TILE + i * rows;
+            if (pos >= piece.len) continue;
+            const int j = pos / p.page_block_size, e = ld_in(p.table + (int64_t)piece.req * p.table_stride + j);
+            if (e < 0 || e >= p.num_pages) continue;
+            w.page[u] = e;
+            w.in[u] = pos - j * p.page_block_size;
+            // rows [i rows, + k) of the block
+            const int k = min(piece.len - pos, rows), at = i * rows;
+            if (rows >= 32) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int n = min(max(at + k - 32 * v, 0), 32);
+                    if (32 * v >= at && n > 0) mine[v] |= n == 32 ? ~0u : (1u << n) - 1u;
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if ((at >> 5) == v) mine[v] |= ((1u << k) - 1u) << (at & 31);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) w.valid[v] = __reduce_or_sync(0xffffffffu, mine[v]);
+        if (++b == piece.b1) {
+            more = piece.next(p);
+            b = -1;
+        }
+    }
+};
+
+// one(copy's number, its page, its first row in the page) for copies [i0, i1) that are there, in one lane with operands that are the same in all.
+template <class F> __device__ __forceinline__ void each_copy(const BlockPlaces& w, int i0, int i1, F&& one) {
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+        const int u = i >> 5;
+        const int pg = u == 0 ? w.page[0] : u == 1 ? w.page[1] : u == 2 ? w.page[2] : w.page[3], in = u == 0 ? w.in[0] : u == 1 ? w.in[1] : u == 2 ? w.in[2] : w.in[3];
+        const int e = __shfl_sync(0xffffffffu, pg, i & 31), y = __shfl_sync(0xffffffffu, in, i & 31);
+        if (e >= 0 && elect_one()) one(i, e, y);
+    }
+    __syncwarp();
+}
+// How many of copies [i0, i1) there are.
+__device__ __forceinline__ uint32_t copies_of(const BlockPlaces& w, int i0, int i1) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int i = (int)(threadIdx.x & 31) + 32 * u;
+        n += (uint32_t)__popc(__ballot_sync(0xffffffffu, w.page[u] >= 0 && i >= i0 && i < i1));
+    }
+    return n;
+}
+
+// Values that are no numbers, replaced by zeros.
+template <bool F16> __device__ __forceinline__ uint32_t numbers_only(uint32_t x) {
+    constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+    if ((x & E) == E) x &= 0xffff0000u;
+    if ((x & (E << 16)) == (E << 16)) x &= 0x0000ffffu;
+    return x;
+}
+
+template <bool F16> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PP_THREADS, 1)
+attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* sm = smem_raw + (base - raw);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + PPMISC_OFF + 4);
+    const uint32_t abort_addr = base + PPMISC_OFF + 4;
+    auto bar = [&](int i) -> uint32_t { return base + PPB_OFF + 8u * i; };
+    auto barp = [&](int i) -> uint32_t { return mapa_shared(bar(i), 0); };     // the even CTA's
+    auto commit_both = [&](int i) {
+        tc_commit_pair(bar(i));
+        tc_commit_pair(mapa_shared(bar(i), 1));
+    };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int part = blockIdx.x >> 1, group0 = (int)blockIdx.y * PP_TILE, row0 = group0 + 64 * (int)rank;
+    const int live = min(max(p.rows - row0, 0), 64);
+
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(bar(PB_KFULL + i), 1);
+            mbar_init(bar(PB_KPEERP + i), 1);
+            mbar_init(bar(PB_KFREE + i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(PB_VFULL + i), 2);
+            mbar_init(bar(PB_VPEERP + i), 1);
+            mbar_init(bar(PB_VFREE + i), 1);
+            mbar_init(bar(PB_SREADY + i), 1);
+            mbar_init(bar(PB_SFREEP + i), 2 * PP_SM_WARPS);
+        }
+        mbar_init(bar(PB_PREADYP), 2 * PP_SM_WARPS);
+        mbar_init(bar(PB_PVDONE), 1);
+        mbar_init(bar(PB_QFREE), 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == PP_S_WARP) { tmem_alloc_pair(base + PPMISC_OFF, 512); tmem_relinquish_pair(); }
+    cluster_sync_all();          // the partner's barriers exist before anything arrives on them
+    grid_dep_wait();
+    grid_dep_launch();
+    Pieces<PP_TILE> piece = partition_of<PP_TILE>(p, part, reinterpret_cast<long long*>(sm + PPW_OFF), PP_WARPS);
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + PPMISC_OFF);
+
+    if (warp < PP_SM_WARPS) {
+        // =================================================================== softmax + epilogue
+        const int quarter = warp & 3, ch = warp >> 2, grp = quarter & 1, thalf = quarter >> 1;
+        const int hrow = 32 * grp + lane, xpart = 2 * thalf + ch;
+        const int col0 = 64 * thalf + 32 * ch;                    // the thread's rows of a block: [col0, + 32)
+        const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+        const float c = p.sm_scale * LOG2E;
+        float* xch = reinterpret_cast<float*>(sm + PPX_OFF);
+        const uint32_t s_free = barp(PB_SFREEP), p_ready = barp(PB_PREADYP);
+        uint32_t it = 0;
+        bool dead = false, stop = false;
+        while (!stop && piece.next(p)) {
+            const bool whole = piece.whole();
+            if (group0 == 0 && rank == 0 && tid == 0 && piece.b0 == 0) piece.write_span(p, part);
+            const int see = paged_sees(p, piece.len, row0 + hrow);
+            const int see_least = paged_sees(p, piece.len, group0);       // of the pair's query rows
+            float m = -INFINITY, l = 0.f;
+            for (int b = piece.b0; b < piece.b1; ++b, ++it) {
+                const uint32_t st = it & 1;
+                if (!dead) dead = !mbar_wait_lean(bar(PB_SREADY + st), (it >> 1) & 1u, abort_addr, WQ_SREADY);
+                uint32_t sv[32];
+                float mx = -INFINITY;
+                const int pos0 = b * PP_TILE;
+                bool plain = true;                                // all rows are there and seen by all query rows
+                const uint4 valid = *reinterpret_cast<const uint4*>(sm + PPY_OFF + 16 * (it & 3));
+                if (!dead) {
+                    tc_fence_after();
+                    tmem_ld32(lane_addr + PPT_S + 64 * st + 32 * ch, sv);
+                    plain = (valid.x & valid.y & valid.z & valid.w) == ~0u && pos0 <= see_least - PP_TILE;
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(s_free + 8 * st);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * c);
+                    if (!plain) {
+                        uint32_t seen = col0 < 32 ? valid.x : col0 < 64 ? valid.y : col0 < 96 ? valid.z : valid.w;
+                        const int n = see - pos0 - col0;          // of the thread's 32 rows, those before the query's last
+                        seen = n <= 0 ? 0u : n < 32 ? seen & ((1u << n) - 1u) : seen;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!((seen >> i) & 1u)) sv[i] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(sv[i]));
+                }
+                // The four threads of a query row (in the four warps of a barrier) exchange their maxima only when one of the barrier's rows has
+                // outgrown its running maximum: rare after a request's first blocks.
+                if (named_bar_or(1 + grp, 128, mx > m + PG_TAU || dead)) {
+                    xch[64 * xpart + hrow] = mx;
+                    if (named_bar_or(1 + grp, 128, dead || *abort_flag != 0)) { stop = true; break; }
+                    const float all = fmaxf(fmaxf(xch[hrow], xch[64 + hrow]), fmaxf(xch[128 + hrow], xch[192 + hrow]));
+                    float al = 1.f;
+                    if (all > m + PG_TAU) { al = ex2(m - all); m = all; l *= al; }
+                    if (b > piece.b0 && __any_sync(0xffffffffu, al != 1.f)) {
+                        dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
+                        if (dead) continue;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int d = 0; d < 128; d += 16) {
+                            const uint32_t at = lane_addr + PPT_O + 128 * ch + d;
+                            uint32_t o[16];
+                            tmem_ld16(at, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                            tmem_st16(at, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                const float mm = m == -INFINITY ? 0.f : m;
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float a = ex2(__uint_as_float(sv[2 * i]) - mm), e = ex2(__uint_as_float(sv[2 * i + 1]) - mm);
+                    l += a + e;
+                    w[i] = pack_weights<F16>(a, e);
+                }
+                // the weights of the block before have been read
+                if (it > 0 && !dead) dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
+                if (!plain && !dead) {
+                    // Rows that are not there, and values that are no numbers in rows hidden from some query, would reach queries through
+                    // 0 x V: they are taken out of the stage.  (A query that sees such a row has a weight that is no number.)
+#pragma unroll 1
+                    for (int h = 0; h < 2 && !dead; ++h) dead = !mbar_wait_lean(bar(PB_VFULL + h), it & 1u, abort_addr, WQ_VFULL);
+                    if (!dead) {
+#pragma unroll 1
+                        for (int i = tid; i < PP_TILE * 32; i += PP_SM_WARPS * 32) {
+                            const int r = (i >> 3) & 127, word = r >> 5;
+                            const uint32_t there = word == 0 ? valid.x : word == 1 ? valid.y : word == 2 ? valid.z : valid.w;
+                            uint4* at = reinterpret_cast<uint4*>(sm + PPV_OFF + ((r >> 6) * 4 + (i >> 10)) * G_CHUNK + (r & 63) * 128 + (i & 7) * 16);
+                            if (!((there >> (r & 31)) & 1u)) {
+                                *at = make_uint4(0, 0, 0, 0);
+                            } else if (pos0 + r >= see_least) {
+                                uint4 v = *at;
+                                v.x = numbers_only<F16>(v.x); v.y = numbers_only<F16>(v.y); v.z = numbers_only<F16>(v.z); v.w = numbers_only<F16>(v.w);
+                                *at = v;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(sm + PPP_OFF + thalf * G_CHUNK + gswz((uint32_t)hrow, (uint32_t)(4 * ch + i))) =
+                        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                fence_proxy_async();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(p_ready);
+            }
+            if (stop) break;
+            // ---- epilogue
+            if (piece.b1 > piece.b0 && !dead) dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
+            tc_fence_after();
+            if (named_bar_or(1 + grp, 128, dead || *abort_flag != 0)) { stop = true; break; }     // (the maxima have been read)
+            xch[64 * xpart + hrow] = l;
+            named_bar_sync(1 + grp, 128);
+            l = (xch[hrow] + xch[64 + hrow]) + (xch[128 + hrow] + xch[192 + hrow]);
+            const size_t rec = whole ? (size_t)piece.req : (size_t)(2 * part + (piece.b0 == 0 ? 1 : 0));
+            const size_t row = rec * p.rows + row0 + hrow;
+            float lse = l == 0.f ? NEG_BIG : log2f(l) + m, denom = l;
+            if (whole && p.attn_sink != nullptr && hrow < live) {
+                const float sink2 = ld_in(p.attn_sink + (row0 + hrow) % p.num_heads) * LOG2E;
+                if (l != 0.f) denom += exp2f(sink2 - m);
+                lse = with_sink(lse, sink2);
+            }
+            if (xpart == 0 && hrow < live) (whole ? p.lse : p.lse_part)[row] = lse;
+            const float f = l == 0.f ? 0.f : 1.f / denom;         // 0: nothing is seen, or the sink takes all
+            const size_t at = row * D_V + 256 * thalf + 128 * ch;
+            auto store = [&](auto* dst, auto pack) {              // pack(16 fp32 values): 32-byte sectors
+                const bool sectors = (reinterpret_cast<size_t>(dst) & 31) == 0;
+#pragma unroll 1
+                for (int d = 0; d < 128; d += 16) {
+                    uint32_t o[16];
+                    if (piece.b1 > piece.b0) tmem_ld16(lane_addr + PPT_O + 128 * ch + d, o);
+                    tmem_wait_ld();
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
+                    if (hrow < live) pack(v, dst + d, sectors);
+                }
+            };
+            auto put = [](void* to, const uint32_t (&x)[8], bool sectors) {
+                if (sectors) {
+                    st_global_v8(to, x);
+                } else {
+                    static_cast<uint4*>(to)[0] = make_uint4(x[0], x[1], x[2], x[3]);
+                    static_cast<uint4*>(to)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+                }
+            };
+            if (whole) {
+                store(static_cast<uint16_t*>(p.out) + at, [&](const float (&v)[16], uint16_t* to, bool sectors) {
+                    uint32_t x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = pack_weights<F16>(v[2 * i], v[2 * i + 1]);
+                    put(to, x, sectors);
+                });
+            } else {
+                store(p.o_part + at, [&](const float (&v)[16], float* to, bool sectors) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(v[8 * h + i]);
+                        put(to + 8 * h, x, sectors);
+                    }
+                });
+            }
+            tc_fence_before();
+        }
+    } else if (warp < PP_S_WARP) {
+        // =================================================================== rows into the stages, and the queries
+        const bool is_k = warp < PP_V0;
+        const int g = (warp - PP_K0) & 3, rows = p.copy_rows, half = 64 / rows;        // copies of 64 rows
+        const int h = is_k ? (int)rank : g >> 1;                  // which 64 rows of a block
+        const int c0 = is_k ? 2 * g : 4 * (int)rank + 2 * (g & 1), c1 = is_k && g == 3 ? PP_CHUNKS : c0 + 2;
+        // Where chunk c0 of the warp's rows goes; the barriers that it waits for and fills.
+        const uint32_t dst = is_k ? base + PPK_OFF + c0 * G_CHUNK : base + PPV_OFF + (4 * h + 2 * (g & 1)) * G_CHUNK;
+        const uint32_t full = bar(is_k ? PB_KFULL + g : PB_VFULL + h), free = bar(is_k ? PB_KFREE + g : PB_VFREE + h);
+        BlockWalk walk(p, piece);
+        BlockPlaces w0, w1;
+        uint32_t pieces = 0;
+        bool ok = true;
+        walk.look_up(p, row0, w0);
+        walk.look_up(p, row0, w1);
+        for (uint32_t it = 0; w0.have && ok; ++it) {
+            if (it >= 1) ok = mbar_wait_lean(free, (it - 1) & 1u, abort_addr, is_k ? WQ_KFREE : WQ_VFREE);
+            if (ok && is_k && w0.first && pieces > 0) ok = mbar_wait_lean(bar(PB_QFREE), (pieces - 1) & 1u, abort_addr, WQ_QFREE);
+            if (!ok) break;
+            // (this slot's last readers, the softmax warps four blocks ago, gave their score buffer back before the products that the wait was for)
+            if (is_k && g == 0 && lane == 0)
+                *reinterpret_cast<uint4*>(sm + PPY_OFF + 16 * (it & 3)) = make_uint4(w0.valid[0], w0.valid[1], w0.valid[2], w0.valid[3]);
+            const uint32_t bytes = copies_of(w0, h * half, (h + 1) * half) * (uint32_t)(rows * 128);
+            const bool queries = is_k && w0.first;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(full, (uint32_t)(c1 - c0) * (bytes + (queries ? G_CHUNK : 0u)));
+                if (queries)
+                    for (int ch = c0; ch < c1; ++ch) tma_load_2d(base + PPQ_OFF + ch * G_CHUNK, &q_map, ch * 64, w0.q_row, full);
+            }
+            each_copy(w0, h * half, (h + 1) * half, [&](int i, int e, int y) {
+                for (int ch = c0; ch < c1; ++ch) tma_load_3d(dst + (ch - c0) * G_CHUNK + (i - h * half) * rows * 128, &k_map, ch * 64, y, e, full);
+            });
+            if (w0.first) ++pieces;
+            w0 = w1;
+            walk.look_up(p, row0, w1);
+            // asked into L2 two blocks ahead: what waits for a free stage should not wait for HBM as well
+            if (is_k && w1.have)
+                each_copy(w1, h * half, (h + 1) * half, [&](int, int e, int y) {
+                    for (int ch = c0; ch < c1; ++ch) tma_prefetch_3d(&k_map, ch * 64, y, e);
+                });
+        }
+    } else if (warp == PP_S_WARP) {
+        // =================================================================== scores (odd CTA: its K has landed)
+        constexpr uint32_t idesc = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, false, false, 128, PP_TILE);
+        const uint32_t q_lo = desc_lo(base + PPQ_OFF, 16), k_lo = desc_lo(base + PPK_OFF, 16), k_peer = barp(PB_KPEERP);
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && piece.next(p)) {
+            for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
+                const uint32_t st = it & 1;
+                if (rank == 0 && it >= 2) ok = mbar_wait_lean(bar(PB_SFREEP + st), ((it >> 1) - 1) & 1u, abort_addr, WQ_SFREE);
+#pragma unroll 1
+                for (int g = 0; g < 4 && ok; ++g) {
+                    ok = mbar_wait_lean(bar(PB_KFULL + g), it & 1u, abort_addr, WQ_KFULL);
+                    if (ok && rank == 0) ok = mbar_wait_lean(bar(PB_KPEERP + g), it & 1u, abort_addr, WQ_KPEER);
+                    if (!ok) break;
+                    if (rank != 0) {
+                        if (lane == 0) mbar_arrive_remote(k_peer + 8 * g);
+                        continue;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t qa = q_lo + ((2 * g * G_CHUNK) >> 4), ka = k_lo + ((2 * g * G_CHUNK) >> 4), d = tmem + PPT_S + 64 * st;
+                        mma_pair_f16(d, make_desc(qa, PP_DESC_HI), make_desc(ka, PP_DESC_HI), idesc, g != 0);
+#pragma unroll
+                        for (int k = 1; k < 8; ++k)
+                            mma_pair_f16(d, make_desc(qa + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI),
+                                         make_desc(ka + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI), idesc, true);
+                        if (g == 3) {
+#pragma unroll
+                            for (int k = 8; k < 12; ++k)
+                                mma_pair_f16(d, make_desc(qa + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI),
+                                             make_desc(ka + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI), idesc, true);
+                            commit_both(PB_SREADY + st);
+                            if (b + 1 == piece.b1) commit_both(PB_QFREE);
+                        }
+                        commit_both(PB_KFREE + g);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        // =================================================================== P.V (odd CTA: its V has landed)
+        constexpr uint32_t idesc = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, false, true, 128, 256);
+        const uint32_t p_lo = desc_lo(base + PPP_OFF, 16), v_lo = desc_lo(base + PPV_OFF, G_CHUNK), v_peer = barp(PB_VPEERP);   // V: the next 64 dims lie a chunk further
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && piece.next(p)) {
+            for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
+                if (rank == 0) ok = mbar_wait_lean(bar(PB_PREADYP), it & 1u, abort_addr, WQ_PREADY);
+#pragma unroll 1
+                for (int h = 0; h < 2 && ok; ++h) {
+                    ok = mbar_wait_lean(bar(PB_VFULL + h), it & 1u, abort_addr, WQ_VFULL);
+                    if (ok && rank == 0) ok = mbar_wait_lean(bar(PB_VPEERP + h), it & 1u, abort_addr, WQ_VPEER);
+                    if (!ok) break;
+                    if (rank != 0) {
+                        if (lane == 0) mbar_arrive_remote(v_peer + 8 * h);
+                        continue;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_pair_f16(tmem + PPT_O + 128 * n, make_desc(p_lo + ((h * G_CHUNK + k * 32) >> 4), PP_DESC_HI),
+                                             make_desc(v_lo + (((4 * h + 2 * n) * G_CHUNK + k * 2048) >> 4), PP_DESC_HI), idesc,
+                                             b != piece.b0 || h != 0 || k != 0);
+                        }
+                        commit_both(PB_VFREE + h);
+                        if (h == 1) commit_both(PB_PVDONE);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+
+    if (*abort_flag != 0) {        // a wait gave up: copies and MMAs may still be in flight; give them time to finish
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000) { }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();            // the partner may still arrive on this CTA's barriers until here
+    if (tid == 0 && *abort_flag != 0 && p.status != nullptr) {
+        atomicCAS(p.status, 0, *abort_flag);
+        atomicAdd(p.status + 1, 1);
+        p.status[2] = blockIdx.x;
+    }
+    if (warp == PP_S_WARP) { tc_fence_after(); tmem_dealloc_pair(tmem, 512); }
+}
+
+}  // namespace
+
+int launch_attn_paged_pair(const PagedParams& p, bool f16, const CUtensorMap& q_map, const CUtensorMap& k_map, cudaStream_t stream) {
+    static std::atomic<bool> attr_set[64];
+    const auto kernel = f16 ? attn_paged_pair_kernel<true> : attn_paged_pair_kernel<false>;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return set_error(SMLA_E_SHAPE, "attn_paged_pair_kernel: device ordinal %d not supported", dev);
+    if (!attr_set[dev]) {
+        for (const auto k : {attn_paged_pair_kernel<true>, attn_paged_pair_kernel<false>}) {
+            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PP_SMEM);
+            if (e != cudaSuccess) return set_error((int)e, "attn_paged_pair_kernel: cannot reserve %u bytes of shared memory: %s", PP_SMEM, cudaGetErrorString(e));
+        }
+        attr_set[dev] = true;
+    }
+    launch_dependent(kernel, dim3(2 * p.num_parts, (p.rows + PP_TILE - 1) / PP_TILE), dim3(PP_THREADS), PP_SMEM, stream, p, q_map, k_map);
+    return check_launch("attn_paged_pair_kernel");
+}
+
+}  // namespace smla

@@ -22,5 +22,7 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void*
 
 // The cache as 32-bit words, 164 per row; boxes of 32 words (128 bytes) of one row, 128B swizzle.  0 or an error code.
 int rows_tensor_map(const uint8_t* kv, CUtensorMap* map);
+// paged_pair.cu
+int launch_attn_paged_pair(const PagedParams& p, bool f16, const CUtensorMap& q_map, const CUtensorMap& k_map, cudaStream_t stream);
 
 }  // namespace smla

@@ -69,7 +69,7 @@ const char* smla_status_string(int code) {
         case 61: return "paged attention rows stored"; case 62: return "paged attention rows free"; case 63: return "paged attention s_ready";
         case 64: return "paged attention p_ready"; case 65: return "paged attention pv_done"; case 66: return "paged attention q_free";
         case 67: return "paged attention s_free";
-        case 91: return "paged attention pair k_full"; case 92: return "paged attention pair k_peer"; case 93: return "paged attention pair k_free";
+        case 91: return "paged attention pair k_full"; case 93: return "paged attention pair k_free";
         case 94: return "paged attention pair v_full"; case 95: return "paged attention pair v_peer"; case 96: return "paged attention pair v_free";
         case 97: return "paged attention pair s_ready"; case 98: return "paged attention pair s_free"; case 99: return "paged attention pair p_ready";
         case 100: return "paged attention pair pv_done"; case 101: return "paged attention pair q_free";

@@ -13,9 +13,9 @@
 // What it costs: V comes in beside K (64 KB next to 72 KB per CTA and block, from L2), since a CTA has other dims of other rows in V than
 // in K, and the two fill shared memory: one stage of each, freed and filled again in parts while the products of the others run.
 //
-// Warps: 0-7 softmax and epilogue (thread = one query row x 32 rows of a block), 8-11 bring in K (two or three chunks each) and the queries, 12-15
-// V (64 rows x 128 dims each), 16 issues the score products, 17 those with V: both in the even CTA, in the odd one they pass on that its
-// K and V have landed.  Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
+// Warps: 0-7 softmax and epilogue (thread = one query row x 32 rows of a block), 8 and 9 bring in K and the queries, 10-13 V (64 rows x
+// 128 dims each), 14 issues the score products, 15 those with V: both in the even CTA, in the odd one 15 passes on that its V has landed.
+// Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
 #include "paged_common.cuh"
 #include "rows_map.cuh"
 
@@ -24,7 +24,7 @@ namespace smla {
 namespace {
 
 constexpr int PP_TILE = 128;                      // cache rows of a block, and query rows of a pair
-constexpr int PP_SM_WARPS = 8, PP_K0 = 8, PP_V0 = 12, PP_S_WARP = 16, PP_WARPS = 18, PP_THREADS = PP_WARPS * 32;
+constexpr int PP_SM_WARPS = 8, PP_K0 = 8, PP_V0 = 10, PP_S_WARP = 14, PP_PV_WARP = 15, PP_WARPS = 16, PP_THREADS = PP_WARPS * 32;
 constexpr int PP_CHUNKS = 9;
 
 constexpr uint32_t PPQ_OFF = 0;
@@ -33,11 +33,12 @@ constexpr uint32_t PPV_OFF = PPK_OFF + PP_CHUNKS * G_CHUNK;   // [2 halves of th
 constexpr uint32_t PPP_OFF = PPV_OFF + 8 * G_CHUNK;           // weights: [2 halves of the block's rows][64 query rows][64]
 constexpr uint32_t PPX_OFF = PPP_OFF + 2 * G_CHUNK;           // [4][64] fp32: maxima, then sums, of the four threads of a query row
 constexpr uint32_t PPW_OFF = PPX_OFF + 4 * 64 * 4;            // schedule, 22 words
-constexpr uint32_t PPY_OFF = PPW_OFF + 22 * 8;                // which of a block's rows are there, [4 blocks] 128 bits
-constexpr uint32_t PPB_OFF = PPY_OFF + 4 * 16;
+constexpr uint32_t PPY_OFF = PPW_OFF + 22 * 8;                // which of a block's rows are there, [8 blocks] 128 bits
+constexpr uint32_t PPB_OFF = PPY_OFF + 8 * 16;
 // Barriers; those with a P collect arrivals of both CTAs and are used in the even one only.
-constexpr int PB_KFULL = 0, PB_KPEERP = 4, PB_KFREE = 8, PB_VFULL = 12, PB_VPEERP = 14, PB_VFREE = 16, PB_SREADY = 18, PB_SFREEP = 20, PB_PREADYP = 22,
-              PB_PVDONE = 23, PB_QFREE = 24, PB_N = 25;
+constexpr int PB_KFULLP = 0, PB_KFREE = PB_KFULLP + 4, PB_VFULL = PB_KFREE + 4, PB_VPEERP = PB_VFULL + 2, PB_VFREE = PB_VPEERP + 2,
+              PB_SREADY = PB_VFREE + 2, PB_SFREEP = PB_SREADY + 2, PB_PREADYP = PB_SFREEP + 2, PB_PVDONE = PB_PREADYP + 2, PB_QFREE = PB_PVDONE + 1,
+              PB_N = PB_QFREE + 1;
 constexpr uint32_t PPMISC_OFF = PPB_OFF + PB_N * 8;
 constexpr uint32_t PP_SMEM = (PPMISC_OFF + 8 + 15) / 16 * 16 + 1024;
 static_assert(PP_SMEM <= 227 * 1024, "shared memory budget");
@@ -46,7 +47,7 @@ static_assert(PPY_OFF % 16 == 0 && PPB_OFF % 8 == 0 && PPMISC_OFF % 8 == 0, "ali
 constexpr uint32_t PPT_O = 0, PPT_S = 256;        // tensor memory: O 2 x 128 columns, two score buffers of 64
 constexpr uint32_t PP_DESC_HI = desc_hi(1024, (uint32_t)SWIZZLE_128B);
 
-enum { WQ_KFULL = 91, WQ_KPEER = 92, WQ_KFREE = 93, WQ_VFULL = 94, WQ_VPEER = 95, WQ_VFREE = 96, WQ_SREADY = 97, WQ_SFREE = 98, WQ_PREADY = 99, WQ_PVDONE = 100,
+enum { WQ_KFULL = 91, WQ_KFREE = 93, WQ_VFULL = 94, WQ_VPEER = 95, WQ_VFREE = 96, WQ_SREADY = 97, WQ_SFREE = 98, WQ_PREADY = 99, WQ_PVDONE = 100,
        WQ_QFREE = 101 };
 
 // The block's rows that are there and the pages of their copies: lane i sees to copies i, i + 32, i + 64 and i + 96 of `rows` rows each.
@@ -161,8 +162,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
 
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
-            mbar_init(bar(PB_KFULL + i), 1);
-            mbar_init(bar(PB_KPEERP + i), 1);
+            mbar_init(bar(PB_KFULLP + i), 2);                     // + the bytes of both CTAs' rows
             mbar_init(bar(PB_KFREE + i), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -171,8 +171,8 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
             mbar_init(bar(PB_VFREE + i), 1);
             mbar_init(bar(PB_SREADY + i), 1);
             mbar_init(bar(PB_SFREEP + i), 2 * PP_SM_WARPS);
+            mbar_init(bar(PB_PREADYP + i), PP_SM_WARPS);          // half of the softmax warps of both CTAs: the weights of half of a block's rows
         }
-        mbar_init(bar(PB_PREADYP), 2 * PP_SM_WARPS);
         mbar_init(bar(PB_PVDONE), 1);
         mbar_init(bar(PB_QFREE), 1);
         *abort_flag = 0;
@@ -191,9 +191,12 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
         const int hrow = 32 * grp + lane, xpart = 2 * thalf + ch;
         const int col0 = 64 * thalf + 32 * ch;                    // the thread's rows of a block: [col0, + 32)
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-        const float c = p.sm_scale * LOG2E;
+        // The sign of the softmax scale goes into the scores.  Never 0: rows that are not seen have scores of -inf, and -inf times 0 would be no
+        // number; 2^-62 times any score is far below one step of an exponent.
+        const float c = fmaxf(fabsf(p.sm_scale * LOG2E), 0x1p-62f);
+        const bool negative = p.sm_scale < 0.f;
         float* xch = reinterpret_cast<float*>(sm + PPX_OFF);
-        const uint32_t s_free = barp(PB_SFREEP), p_ready = barp(PB_PREADYP);
+        const uint32_t s_free = barp(PB_SFREEP), p_ready = barp(PB_PREADYP + thalf);
         uint32_t it = 0;
         bool dead = false, stop = false;
         while (!stop && piece.next(p)) {
@@ -209,7 +212,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                 float mx = -INFINITY;
                 const int pos0 = b * PP_TILE;
                 bool plain = true;                                // all rows are there and seen by all query rows
-                const uint4 valid = *reinterpret_cast<const uint4*>(sm + PPY_OFF + 16 * (it & 3));
+                const uint4 valid = *reinterpret_cast<const uint4*>(sm + PPY_OFF + 16 * (it & 7));
                 if (!dead) {
                     tc_fence_after();
                     tmem_ld32(lane_addr + PPT_S + 64 * st + 32 * ch, sv);
@@ -218,8 +221,10 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_remote(s_free + 8 * st);
+                    if (negative) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * c);
+                        for (int i = 0; i < 32; ++i) sv[i] ^= 0x80000000u;
+                    }
                     if (!plain) {
                         uint32_t seen = col0 < 32 ? valid.x : col0 < 64 ? valid.y : col0 < 96 ? valid.z : valid.w;
                         const int n = see - pos0 - col0;          // of the thread's 32 rows, those before the query's last
@@ -229,7 +234,8 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                             if (!((seen >> i) & 1u)) sv[i] = 0xff800000u;
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(sv[i]));
+                    for (int i = 0; i < 32; i += 2) mx = fmaxf(fmaxf(mx, __uint_as_float(sv[i])), __uint_as_float(sv[i + 1]));
+                    mx *= c;
                 }
                 // The four threads of a query row (in the four warps of a barrier) exchange their maxima only when one of the barrier's rows has
                 // outgrown its running maximum: rare after a request's first blocks.
@@ -256,30 +262,30 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                         tmem_wait_st();
                     }
                 }
-                const float mm = m == -INFINITY ? 0.f : m;
+                const float mm = m == -INFINITY ? 0.f : -m;
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float a = ex2(__uint_as_float(sv[2 * i]) - mm), e = ex2(__uint_as_float(sv[2 * i + 1]) - mm);
+                    const float a = ex2(fmaf(__uint_as_float(sv[2 * i]), c, mm)), e = ex2(fmaf(__uint_as_float(sv[2 * i + 1]), c, mm));
                     l += a + e;
                     w[i] = pack_weights<F16>(a, e);
                 }
-                // the weights of the block before have been read
-                if (it > 0 && !dead) dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
+                // The weights of the block before have been read.  (Each half of a block's rows has its own hand-over, so that the weights of one are
+                // stored while the products of the other run: a second buffer does not fit.)
+                if (it > 0 && !dead) dead = !mbar_wait_lean(bar(PB_VFREE + thalf), (it - 1) & 1u, abort_addr, WQ_VFREE);
                 if (!plain && !dead) {
                     // Rows that are not there, and values that are no numbers in rows hidden from some query, would reach queries through
                     // 0 x V: they are taken out of the stage.  (A query that sees such a row has a weight that is no number.)
-#pragma unroll 1
-                    for (int h = 0; h < 2 && !dead; ++h) dead = !mbar_wait_lean(bar(PB_VFULL + h), it & 1u, abort_addr, WQ_VFULL);
+                    dead = !mbar_wait_lean(bar(PB_VFULL + thalf), it & 1u, abort_addr, WQ_VFULL);
                     if (!dead) {
+                        const uint32_t there0 = thalf ? valid.z : valid.x, there1 = thalf ? valid.w : valid.y;
 #pragma unroll 1
-                        for (int i = tid; i < PP_TILE * 32; i += PP_SM_WARPS * 32) {
-                            const int r = (i >> 3) & 127, word = r >> 5;
-                            const uint32_t there = word == 0 ? valid.x : word == 1 ? valid.y : word == 2 ? valid.z : valid.w;
-                            uint4* at = reinterpret_cast<uint4*>(sm + PPV_OFF + ((r >> 6) * 4 + (i >> 10)) * G_CHUNK + (r & 63) * 128 + (i & 7) * 16);
-                            if (!((there >> (r & 31)) & 1u)) {
+                        for (int i = (2 * grp + ch) * 32 + lane; i < 64 * 32; i += 128) {
+                            const int r = (i >> 3) & 63;
+                            uint4* at = reinterpret_cast<uint4*>(sm + PPV_OFF + (4 * thalf + (i >> 9)) * G_CHUNK + r * 128 + (i & 7) * 16);
+                            if (!(((r & 32 ? there1 : there0) >> (r & 31)) & 1u)) {
                                 *at = make_uint4(0, 0, 0, 0);
-                            } else if (pos0 + r >= see_least) {
+                            } else if (pos0 + 64 * thalf + r >= see_least) {
                                 uint4 v = *at;
                                 v.x = numbers_only<F16>(v.x); v.y = numbers_only<F16>(v.y); v.z = numbers_only<F16>(v.z); v.w = numbers_only<F16>(v.w);
                                 *at = v;
@@ -314,131 +320,148 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
             }
             if (xpart == 0 && hrow < live) (whole ? p.lse : p.lse_part)[row] = lse;
             const float f = l == 0.f ? 0.f : 1.f / denom;         // 0: nothing is seen, or the sink takes all
-            const size_t at = row * D_V + 256 * thalf + 128 * ch;
-            auto store = [&](auto* dst, auto pack) {              // pack(16 fp32 values): 32-byte sectors
-                const bool sectors = (reinterpret_cast<size_t>(dst) & 31) == 0;
+            // 32 dims of each of the warp's 32 query rows at a time, through the weights' place in shared memory, so that four (16-bit) or eight
+            // lanes write a row's neighbouring bytes.  Of the place, the two warps of a quarter have what they later write weights to: after
+            // the next barrier of both.
+            uint8_t* stage = sm + PPP_OFF + thalf * G_CHUNK + grp * 4096 + ch * 2048;
+            const int first_row = row0 + 32 * grp, mine = live - 32 * grp;
 #pragma unroll 1
-                for (int d = 0; d < 128; d += 16) {
-                    uint32_t o[16];
-                    if (piece.b1 > piece.b0) tmem_ld16(lane_addr + PPT_O + 128 * ch + d, o);
-                    tmem_wait_ld();
-                    float v[16];
+            for (int d = 0; d < 128; d += 32) {
+                uint32_t o[32];
+                if (piece.b1 > piece.b0) tmem_ld32(lane_addr + PPT_O + 128 * ch + d, o);
+                tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
-                    if (hrow < live) pack(v, dst + d, sectors);
-                }
-            };
-            auto put = [](void* to, const uint32_t (&x)[8], bool sectors) {
-                if (sectors) {
-                    st_global_v8(to, x);
-                } else {
-                    static_cast<uint4*>(to)[0] = make_uint4(x[0], x[1], x[2], x[3]);
-                    static_cast<uint4*>(to)[1] = make_uint4(x[4], x[5], x[6], x[7]);
-                }
-            };
-            if (whole) {
-                store(static_cast<uint16_t*>(p.out) + at, [&](const float (&v)[16], uint16_t* to, bool sectors) {
-                    uint32_t x[8];
+                for (int i = 0; i < 32; ++i) o[i] = f == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * f);
+                const size_t at = (rec * p.rows + first_row) * D_V + 256 * thalf + 128 * ch + d;
+                if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = pack_weights<F16>(v[2 * i], v[2 * i + 1]);
-                    put(to, x, sectors);
-                });
-            } else {
-                store(p.o_part + at, [&](const float (&v)[16], float* to, bool sectors) {
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                            make_uint4(pack_weights<F16>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])), pack_weights<F16>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
+                                       pack_weights<F16>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])), pack_weights<F16>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
+                    __syncwarp();
+                    uint8_t* dst = reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at) + (lane & 3) * 16;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t x[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(v[8 * h + i]);
-                        put(to + 8 * h, x, sectors);
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 8 * j + (lane >> 2);
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+                        if (r < mine) *reinterpret_cast<uint4*>(dst + (size_t)r * (2 * D_V)) = v;
                     }
-                });
+                    __syncwarp();
+                } else {
+                    uint8_t* dst = reinterpret_cast<uint8_t*>(p.o_part + at) + (lane & 7) * 16;
+#pragma unroll
+                    for (int pass = 0; pass < 2; ++pass) {
+                        if ((lane >> 4) == pass) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<uint4*>(stage + gswz((uint32_t)lane & 15u, (uint32_t)i)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = 4 * j + (lane >> 3);
+                            const uint4 v = *reinterpret_cast<const uint4*>(stage + gswz((uint32_t)r, (uint32_t)lane & 7u));
+                            if (16 * pass + r < mine) *reinterpret_cast<uint4*>(dst + (size_t)(16 * pass + r) * (4 * D_V)) = v;
+                        }
+                        __syncwarp();
+                    }
+                }
             }
             tc_fence_before();
         }
     } else if (warp < PP_S_WARP) {
         // =================================================================== rows into the stages, and the queries
+        // K: a warp has the first and third, or the second and fourth, of four groups of two or three chunks; V: two chunks of 64 rows.  A group has
+        // its barriers; the bytes of both CTAs' K go to the even one's.
         const bool is_k = warp < PP_V0;
-        const int g = (warp - PP_K0) & 3, rows = p.copy_rows, half = 64 / rows;        // copies of 64 rows
-        const int h = is_k ? (int)rank : g >> 1;                  // which 64 rows of a block
-        const int c0 = is_k ? 2 * g : 4 * (int)rank + 2 * (g & 1), c1 = is_k && g == 3 ? PP_CHUNKS : c0 + 2;
-        // Where chunk c0 of the warp's rows goes; the barriers that it waits for and fills.
-        const uint32_t dst = is_k ? base + PPK_OFF + c0 * G_CHUNK : base + PPV_OFF + (4 * h + 2 * (g & 1)) * G_CHUNK;
-        const uint32_t full = bar(is_k ? PB_KFULL + g : PB_VFULL + h), free = bar(is_k ? PB_KFREE + g : PB_VFREE + h);
+        const int g = is_k ? warp - PP_K0 : warp - PP_V0, rows = p.copy_rows, half = 64 / rows;        // copies of 64 rows
+        const int h = is_k ? (int)rank : g >> 1, i0 = h * half;   // which 64 rows of a block
         BlockWalk walk(p, piece);
-        BlockPlaces w0, w1;
+        BlockPlaces w;
         uint32_t pieces = 0;
         bool ok = true;
-        walk.look_up(p, row0, w0);
-        walk.look_up(p, row0, w1);
-        for (uint32_t it = 0; w0.have && ok; ++it) {
-            if (it >= 1) ok = mbar_wait_lean(free, (it - 1) & 1u, abort_addr, is_k ? WQ_KFREE : WQ_VFREE);
-            if (ok && is_k && w0.first && pieces > 0) ok = mbar_wait_lean(bar(PB_QFREE), (pieces - 1) & 1u, abort_addr, WQ_QFREE);
-            if (!ok) break;
-            // (this slot's last readers, the softmax warps four blocks ago, gave their score buffer back before the products that the wait was for)
-            if (is_k && g == 0 && lane == 0)
-                *reinterpret_cast<uint4*>(sm + PPY_OFF + 16 * (it & 3)) = make_uint4(w0.valid[0], w0.valid[1], w0.valid[2], w0.valid[3]);
-            const uint32_t bytes = copies_of(w0, h * half, (h + 1) * half) * (uint32_t)(rows * 128);
-            const bool queries = is_k && w0.first;
-            if (elect_one()) {
-                mbar_arrive_expect_tx(full, (uint32_t)(c1 - c0) * (bytes + (queries ? G_CHUNK : 0u)));
-                if (queries)
-                    for (int ch = c0; ch < c1; ++ch) tma_load_2d(base + PPQ_OFF + ch * G_CHUNK, &q_map, ch * 64, w0.q_row, full);
+        walk.look_up(p, row0, w);
+        for (uint32_t it = 0; w.have; ++it) {
+            // What can be done before the wait is; copies of less than 64 rows are handed from lane to lane after it.
+            const uint32_t bytes = copies_of(w, i0, i0 + half) * (uint32_t)(rows * 128) + (is_k && w.first ? G_CHUNK : 0u);       // of a chunk
+            const int e0 = __shfl_sync(0xffffffffu, w.page[0], i0 & 31), y0 = __shfl_sync(0xffffffffu, w.in[0], i0 & 31);
+            if (is_k) {
+                // (the slot's last readers, the softmax warps eight blocks ago, gave their score buffer back long before)
+                if (g == 0 && lane == 0)
+                    *reinterpret_cast<uint4*>(sm + PPY_OFF + 16 * (it & 7)) = make_uint4(w.valid[0], w.valid[1], w.valid[2], w.valid[3]);
+                if (w.first && pieces > 0) ok = mbar_wait_lean(bar(PB_QFREE), (pieces - 1) & 1u, abort_addr, WQ_QFREE);
             }
-            each_copy(w0, h * half, (h + 1) * half, [&](int i, int e, int y) {
-                for (int ch = c0; ch < c1; ++ch) tma_load_3d(dst + (ch - c0) * G_CHUNK + (i - h * half) * rows * 128, &k_map, ch * 64, y, e, full);
-            });
-            if (w0.first) ++pieces;
-            w0 = w1;
-            walk.look_up(p, row0, w1);
-            // asked into L2 two blocks ahead: what waits for a free stage should not wait for HBM as well
-            if (is_k && w1.have)
-                each_copy(w1, h * half, (h + 1) * half, [&](int, int e, int y) {
-                    for (int ch = c0; ch < c1; ++ch) tma_prefetch_3d(&k_map, ch * 64, y, e);
+#pragma unroll 1
+            for (int n = g; n < 4 && ok; n += is_k ? 2 : 4) {
+                const int c0 = is_k ? 2 * n : 4 * (int)rank + 2 * (g & 1), c1 = is_k && n == 3 ? PP_CHUNKS : c0 + 2;
+                const uint32_t dst = is_k ? base + PPK_OFF + c0 * G_CHUNK : base + PPV_OFF + (4 * h + 2 * (g & 1)) * G_CHUNK;
+                const uint32_t full = is_k ? barp(PB_KFULLP + n) : mapa_shared(bar(PB_VFULL + h), rank);
+                if (it >= 1) ok = mbar_wait_lean(bar(is_k ? PB_KFREE + n : PB_VFREE + h), (it - 1) & 1u, abort_addr, is_k ? WQ_KFREE : WQ_VFREE);
+                if (!ok) break;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx_remote(full, (uint32_t)(c1 - c0) * bytes);
+                    if (half == 1 && e0 >= 0) {
+#pragma unroll 1
+                        for (int ch = c0; ch < c1; ++ch) tma_load_3d_pair(dst + (ch - c0) * G_CHUNK, &k_map, ch * 64, y0, e0, full);
+                    }
+                    if (is_k && w.first) {
+#pragma unroll 1
+                        for (int ch = c0; ch < c1; ++ch) tma_load_2d_pair(base + PPQ_OFF + ch * G_CHUNK, &q_map, ch * 64, w.q_row, full);
+                    }
+                }
+                __syncwarp();
+                if (half > 1)
+                    each_copy(w, i0, i0 + half, [&](int i, int e, int y) {
+#pragma unroll 1
+                        for (int ch = c0; ch < c1; ++ch) tma_load_3d_pair(dst + (ch - c0) * G_CHUNK + (i - i0) * rows * 128, &k_map, ch * 64, y, e, full);
+                    });
+            }
+            if (!ok) break;
+            if (w.first) ++pieces;
+            // The next block's places, and its rows asked into L2: what waits for a free stage should not wait for HBM as well.
+            walk.look_up(p, row0, w);
+            if (is_k && w.have)
+                each_copy(w, i0, i0 + half, [&](int, int e, int y) {
+#pragma unroll 1
+                    for (int ch = g; ch < PP_CHUNKS; ch += 2) tma_prefetch_3d(&k_map, ch * 64, y, e);
                 });
         }
     } else if (warp == PP_S_WARP) {
-        // =================================================================== scores (odd CTA: its K has landed)
+        // =================================================================== scores (even CTA)
         constexpr uint32_t idesc = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, false, false, 128, PP_TILE);
-        const uint32_t q_lo = desc_lo(base + PPQ_OFF, 16), k_lo = desc_lo(base + PPK_OFF, 16), k_peer = barp(PB_KPEERP);
+        const uint32_t q_lo = desc_lo(base + PPQ_OFF, 16), k_lo = desc_lo(base + PPK_OFF, 16);
         uint32_t it = 0;
-        bool ok = true;
+        bool ok = rank == 0;
         while (ok && piece.next(p)) {
             for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
                 const uint32_t st = it & 1;
-                if (rank == 0 && it >= 2) ok = mbar_wait_lean(bar(PB_SFREEP + st), ((it >> 1) - 1) & 1u, abort_addr, WQ_SFREE);
+                if (it >= 2) ok = mbar_wait_lean(bar(PB_SFREEP + st), ((it >> 1) - 1) & 1u, abort_addr, WQ_SFREE);
 #pragma unroll 1
                 for (int g = 0; g < 4 && ok; ++g) {
-                    ok = mbar_wait_lean(bar(PB_KFULL + g), it & 1u, abort_addr, WQ_KFULL);
-                    if (ok && rank == 0) ok = mbar_wait_lean(bar(PB_KPEERP + g), it & 1u, abort_addr, WQ_KPEER);
+                    ok = mbar_wait_lean(bar(PB_KFULLP + g), it & 1u, abort_addr, WQ_KFULL);
                     if (!ok) break;
-                    if (rank != 0) {
-                        if (lane == 0) mbar_arrive_remote(k_peer + 8 * g);
-                        continue;
-                    }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t qa = q_lo + ((2 * g * G_CHUNK) >> 4), ka = k_lo + ((2 * g * G_CHUNK) >> 4), d = tmem + PPT_S + 64 * st;
-                        mma_pair_f16(d, make_desc(qa, PP_DESC_HI), make_desc(ka, PP_DESC_HI), idesc, g != 0);
+                        const uint32_t d = tmem + PPT_S + 64 * st;
+#pragma unroll 1
+                        for (int ch = 2 * g; ch < (g == 3 ? PP_CHUNKS : 2 * g + 2); ++ch) {
+                            const uint32_t qa = q_lo + ((ch * G_CHUNK) >> 4), ka = k_lo + ((ch * G_CHUNK) >> 4);
 #pragma unroll
-                        for (int k = 1; k < 8; ++k)
-                            mma_pair_f16(d, make_desc(qa + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI),
-                                         make_desc(ka + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI), idesc, true);
+                            for (int k = 0; k < 4; ++k)
+                                mma_pair_f16(d, make_desc(qa + 2 * k, PP_DESC_HI), make_desc(ka + 2 * k, PP_DESC_HI), idesc, (ch | k) != 0);
+                        }
+                        commit_both(PB_KFREE + g);
                         if (g == 3) {
-#pragma unroll
-                            for (int k = 8; k < 12; ++k)
-                                mma_pair_f16(d, make_desc(qa + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI),
-                                             make_desc(ka + (((k >> 2) * G_CHUNK + (k & 3) * 32) >> 4), PP_DESC_HI), idesc, true);
                             commit_both(PB_SREADY + st);
                             if (b + 1 == piece.b1) commit_both(PB_QFREE);
                         }
-                        commit_both(PB_KFREE + g);
                     }
                     __syncwarp();
                 }
             }
         }
-    } else {
+    } else if (warp == PP_PV_WARP) {
         // =================================================================== P.V (odd CTA: its V has landed)
         constexpr uint32_t idesc = instr_desc(F16 ? FMT_F16 : FMT_BF16, F16 ? FMT_F16 : FMT_BF16, false, true, 128, 256);
         const uint32_t p_lo = desc_lo(base + PPP_OFF, 16), v_lo = desc_lo(base + PPV_OFF, G_CHUNK), v_peer = barp(PB_VPEERP);   // V: the next 64 dims lie a chunk further
@@ -446,11 +469,11 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
         bool ok = true;
         while (ok && piece.next(p)) {
             for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
-                if (rank == 0) ok = mbar_wait_lean(bar(PB_PREADYP), it & 1u, abort_addr, WQ_PREADY);
 #pragma unroll 1
                 for (int h = 0; h < 2 && ok; ++h) {
                     ok = mbar_wait_lean(bar(PB_VFULL + h), it & 1u, abort_addr, WQ_VFULL);
                     if (ok && rank == 0) ok = mbar_wait_lean(bar(PB_VPEERP + h), it & 1u, abort_addr, WQ_VPEER);
+                    if (ok && rank == 0) ok = mbar_wait_lean(bar(PB_PREADYP + h), it & 1u, abort_addr, WQ_PREADY);
                     if (!ok) break;
                     if (rank != 0) {
                         if (lane == 0) mbar_arrive_remote(v_peer + 8 * h);

@@ -203,6 +203,20 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tensor_map
                  ::"r"(dst), "l"(tensor_map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
+// Loads the box into this CTA's shared memory; the barrier, a shared::cluster address, may be the partner's.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tensor_map, int x, int y, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(tensor_map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tensor_map, int x, int y, int z, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(tensor_map), "r"(x), "r"(y), "r"(z), "r"(cluster_bar) : "memory");
+}
+// Expects bytes and arrives on a barrier of either CTA of the cluster.
+__device__ __forceinline__ void mbar_arrive_expect_tx_remote(uint32_t cluster_bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes) : "memory");
+}
+
 // Makes generic-proxy writes to shared memory visible to the async proxy (tcgen05.mma operands).
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -34,7 +34,8 @@ __host__ __device__ constexpr bool packed_rows(int layout) { return layout == SM
 __host__ __device__ constexpr int load_warps(int layout) { return packed_rows(layout) ? 8 : 4; }
 __host__ __device__ constexpr int paged_threads(int layout) { return packed_rows(layout) ? 640 : 448; }       // (packed: whole groups of four warps)
 // registers of the packed layouts' instances, which the loading warps take from the others
-constexpr int PG_REGS_LAUNCH = 96, PG_REGS_SOFTMAX = 88, PG_REGS_LOAD = 120, PG_REGS_MMA = 48;
+constexpr int PG_REGS_LAUNCH = 96, PG_REGS_SOFTMAX = 96, PG_REGS_LOAD = 112, PG_REGS_MMA = 48;
+static_assert(PG_REGS_SOFTMAX == PG_REGS_LAUNCH && PG_REGS_LOAD >= PG_REGS_LAUNCH && PG_REGS_MMA <= PG_REGS_LAUNCH, "who gives registers and who takes");
 static_assert(PG_SM_WARPS * 32 * PG_REGS_SOFTMAX + 8 * 32 * PG_REGS_LOAD + 4 * 32 * PG_REGS_MMA <= 640 * PG_REGS_LAUNCH, "register budgets exceed what the CTA owns");
 
 constexpr uint32_t G_STAGE = 9 * G_CHUNK;
@@ -45,8 +46,8 @@ constexpr uint32_t GV_OFF = GP_OFF + G_CHUNK;                 // validity: a bit
 constexpr uint32_t GN_OFF = GV_OFF + 16;                      // rows that some query must not see and whose values are no numbers
 constexpr uint32_t GA_OFF = GN_OFF + 16;                      // [64] fp32: rescale factors, then 1 / denominator
 constexpr uint32_t GX_OFF = GA_OFF + PG_ROWS * 4;             // [2][64] fp32: maxima, then sums, of the two halves of a block's rows
-constexpr uint32_t GW_OFF = GX_OFF + 2 * PG_ROWS * 4;         // schedule: block scan [20] int64, start int64, request
-constexpr uint32_t GB_OFF = GW_OFF + 22 * 8;
+constexpr uint32_t GW_OFF = GX_OFF + 2 * PG_ROWS * 4;         // schedule
+constexpr uint32_t GB_OFF = GW_OFF + 24 * 8;
 // KFULL, KFREE: [2 stages][4 groups of dims]
 constexpr int GB_KFULL = 0, GB_KFREE = 8, GB_SREADY = 16, GB_SFREE = 18, GB_PREADY = 20, GB_PVDONE = 21, GB_QFREE = 22, GB_N = 23;
 constexpr uint32_t GMISC_OFF = GB_OFF + GB_N * 8;
@@ -113,9 +114,8 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
     Pieces<64> piece = partition_of<64>(p, part, reinterpret_cast<long long*>(sm + GW_OFF), WARPS);
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + GMISC_OFF);
     if (PACKED) {
-        if (warp < PG_SM_WARPS) setmaxnreg_dec<PG_REGS_SOFTMAX>();
-        else if (warp < S_WARP) setmaxnreg_inc<PG_REGS_LOAD>();
-        else setmaxnreg_dec<PG_REGS_MMA>();
+        if (warp >= S_WARP) setmaxnreg_dec<PG_REGS_MMA>();
+        else if (warp >= LD0) setmaxnreg_inc<PG_REGS_LOAD>();
     }
 
     if (warp < PG_SM_WARPS) {
@@ -134,7 +134,7 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
         while (!stop && piece.next(p)) {
             const bool whole = piece.whole();
             if (row0 == 0 && tid == 0 && piece.b0 == 0) {
-                piece.write_span(p, part);
+                piece.write_span(p, part, reinterpret_cast<long long*>(sm + GW_OFF)[20]);
             }
             const int see_a = paged_sees(p, piece.len, row0 + ra), see_b = paged_sees(p, piece.len, row0 + rb), see_least = paged_sees(p, piece.len, row0);
             float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
@@ -281,7 +281,7 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 const size_t at = (rec * p.rows + row0 + r0) * D_V + 32 * quarter + lane;
                 const int left = live - r0;
                 auto store = [&](auto* dst, auto cvt) {
-#pragma unroll
+#pragma unroll 1
                     for (int d = 0; d < 4; ++d) {
                         uint32_t o[16];
                         if (piece.b1 > piece.b0) tmem_ld16(lane_addr + GT_O + 64 * d + r0, o);
@@ -397,21 +397,25 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
             while (ok && piece.next(p)) {
                 if (piece.b1 == piece.b0) continue;
                 const int32_t* table = p.table + (int64_t)piece.req * p.table_stride;
+                // lane i: where row i % 16 of the warp's rows of a block lies (0: no entry)
+                auto look_up = [&](int b, uint2& scales) {
+                    scales = make_uint2(0u, 0u);
+                    const int pos = b * 64 + 16 * gw + (lane & 15);
+                    if (pos >= piece.len) return 0ull;
+                    const int j = pos / p.page_block_size, page = ld_in(table + j), in = pos - j * p.page_block_size;
+                    if (page < 0 || page >= p.num_pages) return 0ull;
+                    const uint8_t* mine = p.cache + (int64_t)page * p.page_stride;
+                    if (LAYOUT == SMLA_LAYOUT_MODEL1)
+                        scales = ld_in(reinterpret_cast<const uint2*>(mine + (int64_t)p.page_block_size * SMLA_M1_DATA_BYTES + (int64_t)in * 8));
+                    return reinterpret_cast<unsigned long long>(mine + (int64_t)in * (LAYOUT == SMLA_LAYOUT_V32 ? ROW_BYTES : SMLA_M1_DATA_BYTES));
+                };
+                unsigned long long at = 0ull, next_at = 0ull;
+                uint2 sc8 = make_uint2(0u, 0u), next_sc8 = sc8;
+                bool known = false;
                 for (int b = piece.b0; b < piece.b1 && ok; ++b, ++it) {
                     if ((it & 1) != (uint32_t)stage) continue;
-                    // lane i: where row i % 16 of the warp's lies (0: no entry)
-                    unsigned long long at = 0ull;
-                    uint2 sc8 = make_uint2(0u, 0u);
-                    const int pos = b * 64 + 16 * gw + (lane & 15);
-                    if (pos < piece.len) {
-                        const int j = pos / p.page_block_size, page = ld_in(table + j), in = pos - j * p.page_block_size;
-                        if (page >= 0 && page < p.num_pages) {
-                            const uint8_t* mine = p.cache + (int64_t)page * p.page_stride;
-                            if (LAYOUT == SMLA_LAYOUT_MODEL1)
-                                sc8 = ld_in(reinterpret_cast<const uint2*>(mine + (int64_t)p.page_block_size * SMLA_M1_DATA_BYTES + (int64_t)in * 8));
-                            at = reinterpret_cast<unsigned long long>(mine + (int64_t)in * (LAYOUT == SMLA_LAYOUT_V32 ? ROW_BYTES : SMLA_M1_DATA_BYTES));
-                        }
-                    }
+                    if (known) { at = next_at; sc8 = next_sc8; }
+                    else at = look_up(b, sc8);
                     const unsigned bits = __ballot_sync(0xffffffffu, at != 0ull) & 0xffffu;
                     uint4 nope[16], rope[4];
                     float scale[2] = {0.f, 0.f};                  // of row lane / 4 (+ 8), block lane % 4 of 128 dims
@@ -433,6 +437,15 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                         const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, at, 4 * u + (lane >> 3)));
                         rope[u] = make_uint4(0, 0, 0, 0);
                         if (src != nullptr) rope[u] = ld_in_once(reinterpret_cast<const uint4*>(src + ROPE_AT) + (lane & 7));
+                    }
+                    // The warp's next rows, asked into L2 while these are on their way and turned into the stage.
+                    known = b + 2 < piece.b1;
+                    if (known) {
+                        next_at = look_up(b + 2, next_sc8);
+                        if (next_at != 0ull) {
+#pragma unroll
+                            for (int i = 0; i < 3; ++i) prefetch_l2(reinterpret_cast<const uint8_t*>(next_at) + min(128 * (2 * i + (lane >> 4)), ROPE_AT + 127));
+                        }
                     }
                     if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + 4 * stage + 3), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
                     if (!ok) break;

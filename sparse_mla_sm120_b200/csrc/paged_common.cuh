@@ -36,34 +36,32 @@ __device__ __forceinline__ long long paged_share(long long total, int parts) {
 
 // The pieces of a partition, one after the other: request, its rows, and which of its blocks of ROWS rows are the partition's.
 template <int ROWS> struct Pieces {
-    long long lo, hi, start, share;       // the partition's part of the line, where the request begins on it, the length of a part
+    long long lo, hi;                     // the partition's part of the line, from where the request begins on it
     int req, len, nb, b0, b1;
-    bool begun;
     __device__ __forceinline__ bool next(const PagedParams& p) {
         while (true) {
-            if (begun) { start += nb + PG_START; ++req; }
-            begun = true;
-            if (req >= p.batch || start >= hi) return false;
+            if (nb >= 0) { lo -= nb + PG_START; hi -= nb + PG_START; ++req; }
+            if (req >= p.batch || hi <= 0) return false;
             len = paged_length(p, req);
             nb = paged_blocks<ROWS>(len);
-            const long long first = start + PG_START;
-            b0 = (int)max(lo - first, 0ll);
-            b1 = (int)min(hi - first, (long long)nb);
+            b0 = (int)max(lo - PG_START, 0ll);
+            b1 = (int)min(hi - PG_START, (long long)nb);
             if (b1 > b0) return true;
-            if (nb == 0 && first - 1 >= lo && first - 1 < hi) { b0 = b1 = 0; return true; }      // a request without rows: whoever holds its last unit
+            if (nb == 0 && PG_START - 1 >= lo && PG_START - 1 < hi) { b0 = b1 = 0; return true; }      // a request without rows: whoever holds its last unit
         }
     }
     __device__ __forceinline__ bool whole() const { return b0 == 0 && b1 == nb; }
-    // What the merge needs to know, written by the partition that has the request's first block.
-    __device__ __forceinline__ void write_span(const PagedParams& p, int part) const {
-        const long long end = start + PG_START + nb - 1;
-        const int last = whole() ? part : (int)(end <= 0xffffffffll && share <= end ? (unsigned)end / (unsigned)share : end / share);
+    // What the merge needs to know, written by the partition that has the request's first block: the request's last partition.
+    __device__ __forceinline__ void write_span(const PagedParams& p, int part, long long share) const {
+        const long long more = nb + PG_START - hi;        // units behind this partition
+        int last = part;
+        if (!whole() && more > 0) last += more + share <= 0xffffffffll ? (int)((unsigned)(more + share - 1) / (unsigned)share) : (int)((more + share - 1) / share);
         p.spans[req] = make_int2(part, last);
     }
 };
 
-// The partition's part of the line: every thread sums the requests of its share, the block (of `warps` warps) scans the sums.  scan: 22
-// words of shared memory.  Synchronises the block, tensor memory's address included.
+// The partition's part of the line: every thread sums the requests of its share, the block (of `warps` warps) scans the sums.  scan: 23
+// words of shared memory; word 20 has the length of a part afterwards.  Synchronises the block, tensor memory's address included.
 template <int ROWS> __device__ __forceinline__ Pieces<ROWS> partition_of(const PagedParams& p, int part, long long* scan, int warps) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = (p.batch + (int)blockDim.x - 1) / (int)blockDim.x;
@@ -94,15 +92,16 @@ template <int ROWS> __device__ __forceinline__ Pieces<ROWS> partition_of(const P
             if (lo < before + w) break;
             before += w;
         }
-        scan[20] = before;
-        *reinterpret_cast<int*>(scan + 21) = r;
+        scan[21] = before;
+        scan[22] = r;
     }
+    if (tid == 0) scan[20] = share;
     __syncthreads();
     Pieces<ROWS> piece;
-    piece.lo = lo; piece.hi = hi; piece.share = share;
-    piece.start = lo < hi ? scan[20] : 0;
-    piece.req = lo < hi ? *reinterpret_cast<int*>(scan + 21) : p.batch;
-    piece.begun = false;
+    piece.req = lo < hi ? (int)scan[22] : p.batch;
+    piece.lo = lo - scan[21];
+    piece.hi = hi - scan[21];
+    piece.nb = -1;                        // before the first
     return piece;
 }
 

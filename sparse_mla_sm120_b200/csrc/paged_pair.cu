@@ -32,8 +32,8 @@ constexpr uint32_t PPK_OFF = PPQ_OFF + PP_CHUNKS * G_CHUNK;
 constexpr uint32_t PPV_OFF = PPK_OFF + PP_CHUNKS * G_CHUNK;   // [2 halves of the block's rows][4 chunks of 64 dims]
 constexpr uint32_t PPP_OFF = PPV_OFF + 8 * G_CHUNK;           // weights: [2 halves of the block's rows][64 query rows][64]
 constexpr uint32_t PPX_OFF = PPP_OFF + 2 * G_CHUNK;           // [4][64] fp32: maxima, then sums, of the four threads of a query row
-constexpr uint32_t PPW_OFF = PPX_OFF + 4 * 64 * 4;            // schedule, 22 words
-constexpr uint32_t PPY_OFF = PPW_OFF + 22 * 8;                // which of a block's rows are there, [8 blocks] 128 bits
+constexpr uint32_t PPW_OFF = PPX_OFF + 4 * 64 * 4;            // schedule
+constexpr uint32_t PPY_OFF = PPW_OFF + 24 * 8;                // which of a block's rows are there, [8 blocks] 128 bits
 constexpr uint32_t PPB_OFF = PPY_OFF + 8 * 16;
 // Barriers; those with a P collect arrivals of both CTAs and are used in the even one only.
 constexpr int PB_KFULLP = 0, PB_KFREE = PB_KFULLP + 4, PB_VFULL = PB_KFREE + 4, PB_VPEERP = PB_VFULL + 2, PB_VFREE = PB_VPEERP + 2,
@@ -201,7 +201,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
         bool dead = false, stop = false;
         while (!stop && piece.next(p)) {
             const bool whole = piece.whole();
-            if (group0 == 0 && rank == 0 && tid == 0 && piece.b0 == 0) piece.write_span(p, part);
+            if (group0 == 0 && rank == 0 && tid == 0 && piece.b0 == 0) piece.write_span(p, part, reinterpret_cast<long long*>(sm + PPW_OFF)[20]);
             const int see = paged_sees(p, piece.len, row0 + hrow);
             const int see_least = paged_sees(p, piece.len, group0);       // of the pair's query rows
             float m = -INFINITY, l = 0.f;

@@ -186,6 +186,9 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tensor_map
                  ::"r"(dst), "l"(tensor_map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
+// Asks L2 for the line.
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // Asks L2 for the box.
 __device__ __forceinline__ void tma_prefetch_3d(const void* tensor_map, int x, int y, int z) {
     asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(tensor_map), "r"(x), "r"(y), "r"(z) : "memory");

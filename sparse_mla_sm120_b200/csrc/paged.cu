@@ -14,10 +14,21 @@
 //   O^T [4 x 128 dims x rows] += V^T . P^T: A = the same rows read MN-major, B = the weights, a line of 64 rows' weights per query row.
 // O has to be transposed: 64 x 512 fp32 fill half of tensor memory that way, all of it the other way.
 // Warps: 0-7 softmax and epilogue (16 query rows by half of the block's rows each); one that issues the score MMAs and one for P.V; and
-// who brings the rows into two stages of 72 KB: one warp by TMA (16-bit rows), or eight through registers (packed rows: e4m3 x its scale
-// is exact in bf16; four for even blocks, four for odd ones).  A stage is filled and freed in four groups of 128 dims, so that scores
+// who brings the rows into two stages of 72 KB: four warps by TMA (16-bit rows), or eight through registers (packed rows: e4m3 x its scale
+// is exact in bf16 where scales are powers of two, as the writers make them; four for even blocks, four for odd ones).  A stage is filled and freed in four groups of 128 dims, so that scores
 // begin when a quarter of the rows is there, and the next rows come when P.V is through with a quarter.
 // Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
+//
+// Which calls come here: up to 64 query rows per request, and packed rows; more query rows of 16-bit caches go to paged_pair.cu (64
+// requests of up to 8192 rows, 128 heads: 149.6 us here with every row read by two CTAs, 116.2 there).
+// What bounds it: with few query rows the products, whose operands of 64 rows make shared memory the limit (36 + 16 products of a block: 2300
+// cycles for 16 query rows as for 64), of a block's 2700 to 3100; a call of a few blocks is a chain of latencies (entry, lengths, table, rows,
+// four blocks, epilogue, merge: 13.8 us for 1000 rows).  Packed rows: the way through registers, about 5000 cycles for a warp's 16 rows.
+// 48 requests of up to 4096 fp16 rows in pages of 16, two tokens of 16 heads: 44.5 us, 2.9 TB/s; 656-byte rows, 64 requests of up to 8192, 64
+// heads: 107 us; 584-byte, 13 of up to 16384, 128 heads: 91.8 us.
+// What the steps brought (the first version, rows by one warp and one stage of waiting: 52.5, 122.8, 104.7 us): rows by TMA from four warps and
+// stages in quarters 49.1, 118.9, 94.0; rows asked into L2 ahead and a shorter epilogue 44.6, 116.8, 96.8; fewer registers spilled (a spilled
+// register costs hundreds of cycles beside 220 KB of shared memory) and packed rows asked into L2 ahead 44.5, 107.2, 91.8.
 #include "paged_common.cuh"
 #include "rows_map.cuh"
 
@@ -571,17 +582,18 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
     if (warp == S_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// Joins what a request's partitions left, a query row by one warp or, where requests lie in many partitions, by four: warp w sums records w,
-// w + W, ..., four of them asked for at a time.  It is a chain of latencies (one request of 131072 rows in 74 partitions: 64 us with one warp
-// per row and a record at a time, 11 with four), unless there are many rows: then more rows at a time hide it (64 requests of 128 heads
-// in 74 partitions: 25 us with four warps per row).  Requests within one partition are done.  The order of the sums is fixed.
-constexpr int PC_WARPS = 4, PC_AHEAD = 4;
-template <bool F16, int W> __global__ void __launch_bounds__(PC_WARPS * 32) paged_combine_kernel(const PagedParams p) {
+// Joins what a request's partitions left, a query row by one warp or, where requests lie in many partitions, by four or eight: warp w sums records
+// w, w + W, ..., four of them asked for at a time.  It is a chain of latencies (one request of 131072 rows in 74 partitions: 64 us with one warp
+// per row and a record at a time, 11 with four and four records, 9 with eight), unless there are many rows: then more rows at a time hide it
+// (64 requests of 128 heads in 74 partitions: 25 us with four warps per row, 11 with one).  Requests within one partition are done.  The order of the sums is fixed.
+constexpr int PC_ROWS = 4, PC_AHEAD = 4;            // rows of a block where a warp takes one
+__host__ __device__ constexpr int combine_warps(int w) { return w > 1 ? w : PC_ROWS; }
+template <bool F16, int W> __global__ void __launch_bounds__(combine_warps(W) * 32) paged_combine_kernel(const PagedParams p) {
     __shared__ float4 sums[W > 1 ? W - 1 : 1][D_V / 4];
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0;
-    const int64_t id = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * PC_WARPS + (threadIdx.x >> 5);
+    const int64_t id = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * PC_ROWS + (threadIdx.x >> 5);
     if (id >= (int64_t)p.batch * p.rows) return;
     const int req = (int)(id / p.rows), row = (int)(id - (int64_t)req * p.rows);
     const uint2 span = ld_in(reinterpret_cast<const uint2*>(p.spans + req));
@@ -715,11 +727,12 @@ int launch_attn_paged(PagedParams p, int layout, cudaStream_t stream) {
     }
     if (p.num_parts == 1) return 0;                // every request is whole
     const unsigned rows = (unsigned)p.batch * (unsigned)p.rows;
-    const bool many = p.num_parts >= 4 * (int64_t)p.batch;
     typedef void (*Combine)(const PagedParams);
-    const Combine combine = many ? (f16 ? paged_combine_kernel<true, PC_WARPS> : paged_combine_kernel<false, PC_WARPS>)
-                                 : (f16 ? paged_combine_kernel<true, 1> : paged_combine_kernel<false, 1>);
-    launch_dependent(combine, dim3(many ? rows : (rows + PC_WARPS - 1) / PC_WARPS), dim3(PC_WARPS * 32), 0, stream, p);
+    const int warps = p.num_parts >= 16 * (int64_t)p.batch ? 8 : p.num_parts >= 4 * (int64_t)p.batch ? 4 : 1;       // per row
+    const Combine combine = warps == 8   ? (f16 ? paged_combine_kernel<true, 8> : paged_combine_kernel<false, 8>)
+                            : warps == 4 ? (f16 ? paged_combine_kernel<true, 4> : paged_combine_kernel<false, 4>)
+                                         : (f16 ? paged_combine_kernel<true, 1> : paged_combine_kernel<false, 1>);
+    launch_dependent(combine, dim3(warps > 1 ? rows : (rows + PC_ROWS - 1) / PC_ROWS), dim3(combine_warps(warps) * 32), 0, stream, p);
     return check_launch("paged_combine_kernel");
 }
 

@@ -55,6 +55,7 @@ def paged_mla_decode_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     those).  ``causal``: query i of s_q sees rows [0, cache_seqlens - s_q + 1 + i).  Rows in pages that the cache does not have (-1, say)
     count as no entry.  ``num_sm_parts``: partitions that all rows are cut into (default: one per SM and 64 query rows).
     Returns (out [..., H, 512] in q's type, lse [..., H] fp32, base 2 with the sink in it); 0 and -1e30 where a query sees nothing.
-    Exact numerics: products of 16-bit values (the byte layouts' are exact in bf16), fp32 sums and softmax; weights are rounded to 16
+    Exact numerics: products of 16-bit values (the byte layouts' are exact in bf16 where their scales are
+    powers of two, as append_kv_cache and pack_kv_cache write them, else rounded to it), fp32 sums and softmax; weights are rounded to 16
     bits for their product with V."""
     return native().paged_decode(q, kv_cache, block_table, cache_seqlens, sm_scale, d_v, causal, attn_sink, out, num_sm_parts)

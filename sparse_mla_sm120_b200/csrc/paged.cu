@@ -25,10 +25,12 @@
 // cycles for 16 query rows as for 64), of a block's 2700 to 3100; a call of a few blocks is a chain of latencies (entry, lengths, table, rows,
 // four blocks, epilogue, merge: 13.8 us for 1000 rows).  Packed rows: the way through registers, about 5000 cycles for a warp's 16 rows.
 // 48 requests of up to 4096 fp16 rows in pages of 16, two tokens of 16 heads: 44.5 us, 2.9 TB/s; 656-byte rows, 64 requests of up to 8192, 64
-// heads: 107 us; 584-byte, 13 of up to 16384, 128 heads: 91.8 us.
+// heads: 102 us; 584-byte, 13 of up to 16384, 128 heads: 91.9 us.
 // What the steps brought (the first version, rows by one warp and one stage of waiting: 52.5, 122.8, 104.7 us): rows by TMA from four warps and
 // stages in quarters 49.1, 118.9, 94.0; rows asked into L2 ahead and a shorter epilogue 44.6, 116.8, 96.8; fewer registers spilled (a spilled
-// register costs hundreds of cycles beside 220 KB of shared memory) and packed rows asked into L2 ahead 44.5, 107.2, 91.8.
+// register costs hundreds of cycles beside 220 KB of shared memory) and packed rows asked into L2 ahead 44.5, 101.9, 91.9.  Measured and not
+// kept: a packed row's values asked for as soon as those of the block before are in the stage (160, 110: the fence before a stage is handed over
+// waits for the loads).
 #include "paged_common.cuh"
 #include "rows_map.cuh"
 
@@ -45,7 +47,7 @@ __host__ __device__ constexpr bool packed_rows(int layout) { return layout == SM
 __host__ __device__ constexpr int load_warps(int layout) { return packed_rows(layout) ? 8 : 4; }
 __host__ __device__ constexpr int paged_threads(int layout) { return packed_rows(layout) ? 640 : 448; }       // (packed: whole groups of four warps)
 // registers of the packed layouts' instances, which the loading warps take from the others
-constexpr int PG_REGS_LAUNCH = 96, PG_REGS_SOFTMAX = 96, PG_REGS_LOAD = 112, PG_REGS_MMA = 48;
+constexpr int PG_REGS_LAUNCH = 96, PG_REGS_SOFTMAX = 96, PG_REGS_LOAD = 120, PG_REGS_MMA = 48;
 static_assert(PG_REGS_SOFTMAX == PG_REGS_LAUNCH && PG_REGS_LOAD >= PG_REGS_LAUNCH && PG_REGS_MMA <= PG_REGS_LAUNCH, "who gives registers and who takes");
 static_assert(PG_SM_WARPS * 32 * PG_REGS_SOFTMAX + 8 * 32 * PG_REGS_LOAD + 4 * 32 * PG_REGS_MMA <= 640 * PG_REGS_LAUNCH, "register budgets exceed what the CTA owns");
 

@@ -139,3 +139,52 @@ def test_many_requests():
     q, cache, table, n, scale = _case("bf16", lengths, 1, 66, 16, 92)
     out, lse = _run(q, cache, table, n, scale)
     P.check_attention(out, lse, q, cache, table, n, scale, False)
+
+
+@pytest.mark.parametrize("heads", [16, 128])
+def test_a_scale_that_is_no_number(heads):
+    q, cache, table, n, _ = _case("bf16", [70, 0], 1, heads, 64, 101)
+    out, lse = _run(q, cache, table, n, float("nan"))
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
+    assert bool((out[1] == 0).all()) and bool((lse[1] == -1e30).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_captured_step(kind):
+    """Appends and attention of 128 heads as one graph that replays over growing contexts."""
+    from sparse_mla_sm120_b200 import paged
+    g = torch.Generator().manual_seed(111)
+    dt, page, heads, steps = P.DTYPE[kind], 64, 128, 4
+    cache = P.make_cache(kind, 14, page, 112).to(DEV)
+    lengths = torch.tensor([509, 127], dtype=torch.int32, device=DEV)
+    table = P.table_of([520, 140], page, 14, 113).to(DEV)
+    cs = P.rotary_table(600).to(DEV)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dt).to(DEV)
+    down, q, q_pe = rand(2, 576), rand(2, 1, heads, 576), rand(2, heads, 64)
+    slots, pos = torch.zeros(2, dtype=torch.int64, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+
+    def step():
+        paged.append_kv_cache(down[:, :512], down[:, 512:], cache, slots, pos, cs, q_pe=q_pe, q_out=q[:, 0, :, 512:])
+        return paged.paged_mla_decode_fwd(q, cache, table, lengths, 576 ** -0.5)
+
+    def place():
+        pos.copy_(lengths - 1)
+        slots.copy_(table.long().gather(1, (pos // page).unsqueeze(1)).squeeze(1) * page + pos % page)
+    place()
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out, lse = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(steps):
+        lengths += 1
+        place()
+        for buffer in (down, q, q_pe):
+            buffer.copy_(torch.randn(buffer.shape, generator=g).to(dt))
+        graph.replay()
+        torch.cuda.synchronize()
+        P.check_attention(out, lse, q, cache, table, lengths, 576 ** -0.5, False)
+        turned = orc.rotate_ref(q_pe.cpu(), cs.cpu(), pos.cpu(), True)
+        assert float((q[:, 0, :, 512:].cpu().double() - turned).abs().max()) <= P.HALF_STEP[dt] * float(turned.abs().max()) + 1e-5

@@ -254,20 +254,26 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                     if (all > m + PG_TAU) { al = ex2(m - all); m = all; l *= al; }
                     if (b > piece.b0 && __any_sync(0xffffffffu, al != 1.f)) {
                         dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
-                        if (dead) continue;
-                        tc_fence_after();
+                        if (!dead) {
+                            tc_fence_after();
 #pragma unroll 1
-                        for (int d = 0; d < 128; d += 16) {
-                            const uint32_t at = lane_addr + PPT_O + 128 * ch + d;
-                            uint32_t o[16];
-                            tmem_ld16(at, o);
-                            tmem_wait_ld();
+                            for (int d = 0; d < 128; d += 16) {
+                                const uint32_t at = lane_addr + PPT_O + 128 * ch + d;
+                                uint32_t o[16];
+                                tmem_ld16(at, o);
+                                tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                            tmem_st16(at, o);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                                tmem_st16(at, o);
+                            }
+                            tmem_wait_st();
                         }
-                        tmem_wait_st();
                     }
+                    // The products of either half of the block's rows add to all lanes of O and begin when the warps of that half have
+                    // arrived: none of them does before all four have rescaled.
+                    tc_fence_before();
+                    if (named_bar_or(1 + grp, 128, dead)) { stop = true; break; }
+                    tc_fence_after();
                 }
                 const float mm = m == -INFINITY ? 0.f : -m;
                 uint32_t w[16];

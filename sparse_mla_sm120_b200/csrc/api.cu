@@ -72,7 +72,7 @@ const char* smla_status_string(int code) {
         case 91: return "paged attention pair k_full"; case 93: return "paged attention pair k_free";
         case 94: return "paged attention pair v_full"; case 95: return "paged attention pair v_peer"; case 96: return "paged attention pair v_free";
         case 97: return "paged attention pair s_ready"; case 98: return "paged attention pair s_free"; case 99: return "paged attention pair p_ready";
-        case 100: return "paged attention pair pv_done"; case 101: return "paged attention pair q_free";
+        case 101: return "paged attention pair q_free";
         case 51: return "attention tile k_full"; case 52: return "attention tile rope_full"; case 53: return "attention tile k_free";
         case 54: return "attention tile s_ready"; case 55: return "attention tile s_free"; case 56: return "attention tile scales";
         case 57: return "attention tile p_ready"; case 58: return "attention tile pv_done"; case 59: return "attention tile q_ready";

@@ -44,7 +44,7 @@ constexpr uint32_t PPY_OFF = PPW_OFF + 24 * 8;                // which of a bloc
 constexpr uint32_t PPB_OFF = PPY_OFF + 8 * 16;
 // Barriers; those with a P collect arrivals of both CTAs and are used in the even one only.
 constexpr int PB_KFULLP = 0, PB_KFREE = PB_KFULLP + 4, PB_VFULL = PB_KFREE + 4, PB_VPEERP = PB_VFULL + 2, PB_VFREE = PB_VPEERP + 2,
-              PB_SREADY = PB_VFREE + 2, PB_SFREEP = PB_SREADY + 2, PB_PREADYP = PB_SFREEP + 2, PB_PVDONE = PB_PREADYP + 2, PB_QFREE = PB_PVDONE + 1,
+              PB_SREADY = PB_VFREE + 2, PB_SFREEP = PB_SREADY + 2, PB_PREADYP = PB_SFREEP + 2, PB_QFREE = PB_PREADYP + 2,
               PB_N = PB_QFREE + 1;
 constexpr uint32_t PPMISC_OFF = PPB_OFF + PB_N * 8;
 constexpr uint32_t PP_SMEM = (PPMISC_OFF + 8 + 15) / 16 * 16 + 1024;
@@ -54,7 +54,7 @@ static_assert(PPY_OFF % 16 == 0 && PPB_OFF % 8 == 0 && PPMISC_OFF % 8 == 0, "ali
 constexpr uint32_t PPT_O = 0, PPT_S = 256;        // tensor memory: O 2 x 128 columns, two score buffers of 64
 constexpr uint32_t PP_DESC_HI = desc_hi(1024, (uint32_t)SWIZZLE_128B);
 
-enum { WQ_KFULL = 91, WQ_KFREE = 93, WQ_VFULL = 94, WQ_VPEER = 95, WQ_VFREE = 96, WQ_SREADY = 97, WQ_SFREE = 98, WQ_PREADY = 99, WQ_PVDONE = 100,
+enum { WQ_KFULL = 91, WQ_KFREE = 93, WQ_VFULL = 94, WQ_VPEER = 95, WQ_VFREE = 96, WQ_SREADY = 97, WQ_SFREE = 98, WQ_PREADY = 99,
        WQ_QFREE = 101 };
 
 // The block's rows that are there and the pages of their copies: lane i sees to copies i, i + 32, i + 64 and i + 96 of `rows` rows each.
@@ -180,7 +180,6 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
             mbar_init(bar(PB_SFREEP + i), 2 * PP_SM_WARPS);
             mbar_init(bar(PB_PREADYP + i), PP_SM_WARPS);          // half of the softmax warps of both CTAs: the weights of half of a block's rows
         }
-        mbar_init(bar(PB_PVDONE), 1);
         mbar_init(bar(PB_QFREE), 1);
         *abort_flag = 0;
         mbar_init_fence();
@@ -253,7 +252,9 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                     float al = 1.f;
                     if (all > m + PG_TAU) { al = ex2(m - all); m = all; l *= al; }
                     if (b > piece.b0 && __any_sync(0xffffffffu, al != 1.f)) {
-                        dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
+                        // All products of the block before.  (A parity tells a phase from its neighbours only: the phase before this one
+                        // is known to be over, for the thalf 1 warps waited for it ahead of the barriers above.)
+                        dead = !mbar_wait_lean(bar(PB_VFREE + 1), (it - 1) & 1u, abort_addr, WQ_VFREE);
                         if (!dead) {
                             tc_fence_after();
 #pragma unroll 1
@@ -317,11 +318,13 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
             }
             if (stop) break;
             // ---- epilogue
-            if (piece.b1 > piece.b0 && !dead) dead = !mbar_wait_lean(bar(PB_PVDONE), (it - 1) & 1u, abort_addr, WQ_PVDONE);
-            tc_fence_after();
-            if (named_bar_or(1 + grp, 128, dead || *abort_flag != 0)) { stop = true; break; }     // (the maxima have been read)
+            // Behind this barrier the maxima have been read, and the thalf 1 warps have waited for half 1 of the block before the last: the
+            // parity that is asked for next is the last block's.
+            if (named_bar_or(1 + grp, 128, dead || *abort_flag != 0)) { stop = true; break; }
+            if (piece.b1 > piece.b0) dead = !mbar_wait_lean(bar(PB_VFREE + 1), (it - 1) & 1u, abort_addr, WQ_VFREE);
             xch[64 * xpart + hrow] = l;
-            named_bar_sync(1 + grp, 128);
+            if (named_bar_or(1 + grp, 128, dead)) { stop = true; break; }
+            tc_fence_after();
             l = (xch[hrow] + xch[64 + hrow]) + (xch[128 + hrow] + xch[192 + hrow]);
             const size_t rec = whole ? (size_t)piece.req : (size_t)(2 * part + (piece.b0 == 0 ? 1 : 0));
             const size_t row = rec * p.rows + row0 + hrow;
@@ -502,8 +505,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                                              make_desc(v_lo + (((4 * h + 2 * n) * G_CHUNK + k * 2048) >> 4), PP_DESC_HI), idesc,
                                              b != piece.b0 || h != 0 || k != 0);
                         }
-                        commit_both(PB_VFREE + h);
-                        if (h == 1) commit_both(PB_PVDONE);
+                        commit_both(PB_VFREE + h);        // (of half 1: all products of the block)
                     }
                     __syncwarp();
                 }

@@ -26,3 +26,20 @@ def test_products_wait_for_every_warp_that_rescales():
     # no way past it: a warp whose wait gave up takes part
     rescale = body[body.index("named_bar_or(1 + grp, 128, mx > m"):body.index("const float mm")]
     assert "continue" not in rescale
+
+
+def test_waits_ask_for_a_phase_next_to_one_that_is_over():
+    """paged_pair.cu: a parity is that of a phase and of the one two phases earlier.  A warp may wait for a barrier only where it knows the
+    phase before to be over: those that softmax warps wait for in every block are, and the others' (half 1 of V, for the warps of half 0)
+    only behind a barrier that the warps of half 1 have passed too."""
+    body = _softmax(_source("paged_pair.cu"))
+    meets = [m.start() for m in re.finditer(r"named_bar_or\(1 \+ grp, 128", body)]
+    waits = re.findall(r"mbar_wait_lean\(bar\((PB_\w+)([^)]*)\)", body)
+    assert waits and {w for w, _ in waits} <= {"PB_SREADY", "PB_VFREE", "PB_VFULL"}
+    for m in re.finditer(r"mbar_wait_lean\(bar\(PB_VFREE \+ 1\)", body):
+        # the last thing before it that several warps do together, or wait for, is a meeting of the four
+        before = body[:m.start()]
+        assert max(i for i in meets if i < m.start()) > before.rindex("mbar_wait_lean")
+    # nothing is read from the accumulator in the epilogue before all four warps have waited
+    epilogue = body[body.rindex("mbar_wait_lean(bar(PB_VFREE + 1)"):]
+    assert epilogue.index("named_bar_or(1 + grp, 128, dead)") < epilogue.index("tc_fence_after();") < epilogue.index("tmem_ld32(")

@@ -56,8 +56,7 @@ constexpr uint32_t GQ_OFF = 0;
 constexpr uint32_t GK_OFF = GQ_OFF + G_STAGE;
 constexpr uint32_t GP_OFF = GK_OFF + 2 * G_STAGE;             // weights [64 query rows][64 rows] 16-bit
 constexpr uint32_t GV_OFF = GP_OFF + G_CHUNK;                 // validity: a bit per row, [2 stages] 64 bits
-constexpr uint32_t GN_OFF = GV_OFF + 16;                      // rows that some query must not see and whose values are no numbers
-constexpr uint32_t GA_OFF = GN_OFF + 16;                      // [64] fp32: rescale factors, then 1 / denominator
+constexpr uint32_t GA_OFF = GV_OFF + 16;                      // [64] fp32: rescale factors, then 1 / denominator
 constexpr uint32_t GX_OFF = GA_OFF + PG_ROWS * 4;             // [2][64] fp32: maxima, then sums, of the two halves of a block's rows
 constexpr uint32_t GW_OFF = GX_OFF + 2 * PG_ROWS * 4;         // schedule
 constexpr uint32_t GB_OFF = GW_OFF + 24 * 8;
@@ -117,7 +116,6 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
         mbar_init(bar(GB_PVDONE), 1);
         mbar_init(bar(GB_QFREE), 1);
         *abort_flag = 0;
-        for (int i = 0; i < 4; ++i) reinterpret_cast<volatile unsigned*>(sm + GN_OFF)[i] = 0u;
         mbar_init_fence();
     }
     if (warp == S_WARP) { tmem_alloc(base + GMISC_OFF, 512); tmem_relinquish(); }
@@ -140,7 +138,6 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
         const float c = p.sm_scale * LOG2E;
         float* factor = reinterpret_cast<float*>(sm + GA_OFF);
         float* other = reinterpret_cast<float*>(sm + GX_OFF);
-        unsigned* none = reinterpret_cast<unsigned*>(sm + GN_OFF);             // [2 stages] 64 bits
         const bool busy = live > 32 * half;                       // the half has columns of O^T
         uint32_t it = 0;
         bool dead = false, stop = false;
@@ -158,7 +155,6 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 float mx_a = -INFINITY, mx_b = -INFINITY;
                 const int pos0 = b * 64;
                 unsigned long long valid = ~0ull;
-                bool odd = false;
                 if (!dead) {
                     tc_fence_after();
                     tmem_ld_16x256b_x4(lane_addr + GT_S + 64 * st + 32 * half, sv);
@@ -171,17 +167,12 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
 #pragma unroll
                         for (int i = 0; i < 16; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * c);
                     } else {
-                        unsigned bad = 0u;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int col = 8 * (i >> 2) + 2 * quad + (i & 1), at = 32 * half + col;
-                            const float x = __uint_as_float(sv[i]) * c;
-                            const bool there = (valid >> at) & 1, seen = there && pos0 + at < ((i & 2) ? see_b : see_a);
-                            if (there && !seen && !(fabsf(x) < INFINITY)) bad |= 1u << col;
-                            sv[i] = __float_as_uint(seen ? x : -INFINITY);
+                            const int at = 32 * half + 8 * (i >> 2) + 2 * quad + (i & 1);
+                            const bool seen = ((valid >> at) & 1) && pos0 + at < ((i & 2) ? see_b : see_a);
+                            sv[i] = __float_as_uint(seen ? __uint_as_float(sv[i]) * c : -INFINITY);
                         }
-                        if (bad) atomicOr(none + 2 * st + half, bad);
-                        odd = bad != 0u;
                     }
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
@@ -196,23 +187,13 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 }
                 if (quad == 0) { other[half * PG_ROWS + ra] = mx_a; other[half * PG_ROWS + rb] = mx_b; }
                 const bool grow = mx_a > m_a + PG_TAU || mx_b > m_b + PG_TAU;                // false while a row has seen nothing
-                if (named_bar_or(1, PG_SM_THREADS, grow || odd || dead || *abort_flag != 0) || valid != ~0ull) {
-                    // rare: a maximum grows, the request's last rows, a hidden row that is no number, or the CTA gives up
+                if (named_bar_or(1, PG_SM_THREADS, grow || dead || *abort_flag != 0)) {
+                    // rare: a maximum grows, or the CTA gives up
                     const float all_a = fmaxf(other[ra], other[PG_ROWS + ra]), all_b = fmaxf(other[rb], other[PG_ROWS + rb]);
                     float al_a = 1.f, al_b = 1.f;
                     if (all_a > m_a + PG_TAU) { al_a = ex2(m_a - all_a); m_a = all_a; l_a *= al_a; }
                     if (all_b > m_b + PG_TAU) { al_b = ex2(m_b - all_b); m_b = all_b; l_b *= al_b; }
                     if (quad == 0 && half == 0) { factor[ra] = al_a; factor[rb] = al_b; }
-                    // Rows that are not there, and rows hidden from some query whose score is no number, would reach queries through
-                    // 0 x V: their values are taken out of the stage.  Queries that see such a row have a weight that is no number.
-                    const unsigned long long hide = ~valid | *reinterpret_cast<volatile unsigned long long*>(none + 2 * st);
-                    if (hide != 0ull && !dead) {
-                        for (int i = tid; i < 64 * CHUNKS * 8; i += PG_SM_THREADS) {
-                            const int r = (i >> 3) & 63;
-                            if ((hide >> r) & 1)
-                                *reinterpret_cast<uint4*>(sm + GK_OFF + st * G_STAGE + (i >> 9) * G_CHUNK + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                    }
                     if (b > piece.b0 && !dead) dead = !mbar_wait_lean(bar(GB_PVDONE), (it - 1) & 1u, abort_addr, WP_PVDONE);
                     if (named_bar_or(1, PG_SM_THREADS, dead || *abort_flag != 0)) { stop = true; break; }
                     if (b > piece.b0 && busy) {
@@ -229,7 +210,6 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                         }
                         tmem_wait_st();
                     }
-                    if (tid == 0) *reinterpret_cast<volatile unsigned long long*>(none + 2 * st) = 0ull;      // (next written two blocks from here)
                     named_bar_sync(1, PG_SM_THREADS);             // the factors and maxima have been read
                 }
                 const float ma = m_a == -INFINITY ? 0.f : m_a, mb = m_b == -INFINITY ? 0.f : m_b;
@@ -245,6 +225,21 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 }
                 // the weights of the block before have been read
                 if (it > 0 && !dead) dead = !mbar_wait_lean(bar(GB_PVDONE), (it - 1) & 1u, abort_addr, WP_PVDONE);
+                if ((valid != ~0ull || pos0 > see_least - 64) && !dead) {
+                    // Rows that are not there, and values that are no numbers in rows hidden from some query, would reach queries through
+                    // 0 x V: they are taken out of the stage, whose scores are done.  (By the rows' values, not by scores, which a query that is
+                    // no number spoils too.  A query that sees such a row has a weight that is no number.)
+#pragma unroll 1
+                    for (int g = 0; g < (PACKED ? 1 : 4) && !dead; ++g)       // over since the scores are there: what copies wrote is read here
+                        dead = !mbar_wait_lean(bar(GB_KFULL + 4 * st + g), (it >> 1) & 1u, abort_addr, WP_KFULL);
+#pragma unroll 1
+                    for (int i = tid; i < 64 * (D_V / 8); i += PG_SM_THREADS) {
+                        const int r = (i >> 3) & 63;
+                        uint4* at = reinterpret_cast<uint4*>(sm + GK_OFF + st * G_STAGE + (i >> 9) * G_CHUNK + r * 128 + (i & 7) * 16);
+                        if (!((valid >> r) & 1)) *at = make_uint4(0, 0, 0, 0);
+                        else if (pos0 + r >= see_least) *at = numbers_only<F16>(*at);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     *reinterpret_cast<uint32_t*>(sm + GP_OFF + gswz((uint32_t)ra, (uint32_t)(4 * half + i)) + 4 * quad) = w[2 * i];

@@ -135,6 +135,17 @@ template <bool F16> __device__ __forceinline__ uint16_t out_bits(float v) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
+// Values that are no numbers, replaced by zeros.
+template <bool F16> __device__ __forceinline__ uint32_t numbers_only(uint32_t x) {
+    constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+    if ((x & E) == E) x &= 0xffff0000u;
+    if ((x & (E << 16)) == (E << 16)) x &= 0x0000ffffu;
+    return x;
+}
+template <bool F16> __device__ __forceinline__ uint4 numbers_only(uint4 v) {
+    return make_uint4(numbers_only<F16>(v.x), numbers_only<F16>(v.y), numbers_only<F16>(v.z), numbers_only<F16>(v.w));
+}
+
 }  // namespace
 
 }  // namespace smla

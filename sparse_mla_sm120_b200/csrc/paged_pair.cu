@@ -140,14 +140,6 @@ __device__ __forceinline__ uint32_t copies_of(const BlockPlaces& w, int i0, int 
     return n;
 }
 
-// Values that are no numbers, replaced by zeros.
-template <bool F16> __device__ __forceinline__ uint32_t numbers_only(uint32_t x) {
-    constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-    if ((x & E) == E) x &= 0xffff0000u;
-    if ((x & (E << 16)) == (E << 16)) x &= 0x0000ffffu;
-    return x;
-}
-
 template <bool F16> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PP_THREADS, 1)
 attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map) {
     extern __shared__ uint8_t smem_raw[];
@@ -300,9 +292,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                             if (!(((r & 32 ? there1 : there0) >> (r & 31)) & 1u)) {
                                 *at = make_uint4(0, 0, 0, 0);
                             } else if (pos0 + 64 * thalf + r >= see_least) {
-                                uint4 v = *at;
-                                v.x = numbers_only<F16>(v.x); v.y = numbers_only<F16>(v.y); v.z = numbers_only<F16>(v.z); v.w = numbers_only<F16>(v.w);
-                                *at = v;
+                                *at = numbers_only<F16>(*at);
                             }
                         }
                     }

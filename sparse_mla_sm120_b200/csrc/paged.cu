@@ -594,7 +594,7 @@ template <bool F16, int W> __global__ void __launch_bounds__(combine_warps(W) * 
     if (id >= (int64_t)p.batch * p.rows) return;
     const int req = (int)(id / p.rows), row = (int)(id - (int64_t)req * p.rows);
     const uint2 span = ld_in(reinterpret_cast<const uint2*>(p.spans + req));
-    const int c0 = (int)span.x, n = (int)span.y - c0 + 1;
+    const int c0 = (int)span.x, n = span_parts(c0, (int)span.y, p.num_parts);
     if (n <= 1) return;
     auto record = [&](int s) { return (size_t)(s == 0 ? 2 * c0 + 1 : 2 * (c0 + s)) * p.rows + row; };
     float4 v[PC_AHEAD][4];

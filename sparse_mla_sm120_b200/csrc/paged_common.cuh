@@ -60,6 +60,10 @@ template <int ROWS> struct Pieces {
     }
 };
 
+// How many partitions a request lies in, by its span; 0 where the words are none.  (A partition whose wait gave up has written no spans: the
+// merge then finds what the scratch held before, and must not read outside of the records.)
+__host__ __device__ inline int span_parts(int first, int last, int num_parts) { return first >= 0 && first <= last && last < num_parts ? last - first + 1 : 0; }
+
 // The partition's part of the line: every thread sums the requests of its share, the block (of `warps` warps) scans the sums.  scan: 23
 // words of shared memory; word 20 has the length of a part afterwards.  Synchronises the block, tensor memory's address included.
 template <int ROWS> __device__ __forceinline__ Pieces<ROWS> partition_of(const PagedParams& p, int part, long long* scan, int warps) {

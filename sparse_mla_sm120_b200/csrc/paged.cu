@@ -379,8 +379,9 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
                 if (it >= 2) ok = mbar_wait_lean(bar(GB_KFREE + 4 * st + g), ((it >> 1) - 1) & 1u, abort_addr, WP_KFREE);
                 if (ok && w0.first && pieces > 0) ok = mbar_wait_lean(bar(GB_QFREE), (pieces - 1) & 1u, abort_addr, WP_QFREE);
                 if (!ok) break;
-                if (g == 0 && lane == 0) *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * st) = ((unsigned long long)w0.v_hi << 32) | w0.v_lo;
                 if (elect_one()) {
+                    // (by the lane whose arrival hands them over)
+                    if (g == 0) *reinterpret_cast<volatile unsigned long long*>(sm + GV_OFF + 8 * st) = ((unsigned long long)w0.v_hi << 32) | w0.v_lo;
                     mbar_arrive_expect_tx(full, (uint32_t)(c1 - c0) * (w0.bytes + (w0.first ? G_CHUNK : 0u)));
                     if (w0.first)
                         for (int ch = c0; ch < c1; ++ch) tma_load_2d(base + GQ_OFF + ch * G_CHUNK, &q_map, ch * 64, w0.q_row, full);

@@ -392,12 +392,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
             // What can be done before the wait is; copies of less than 64 rows are handed from lane to lane after it.
             const uint32_t bytes = copies_of(w, i0, i0 + half) * (uint32_t)(rows * 128) + (is_k && w.first ? G_CHUNK : 0u);       // of a chunk
             const int e0 = __shfl_sync(0xffffffffu, w.page[0], i0 & 31), y0 = __shfl_sync(0xffffffffu, w.in[0], i0 & 31);
-            if (is_k) {
-                // (the slot's last readers, the softmax warps eight blocks ago, gave their score buffer back long before)
-                if (g == 0 && lane == 0)
-                    *reinterpret_cast<uint4*>(sm + PPY_OFF + 16 * (it & 7)) = make_uint4(w.valid[0], w.valid[1], w.valid[2], w.valid[3]);
-                if (w.first && pieces > 0) ok = mbar_wait_lean(bar(PB_QFREE), (pieces - 1) & 1u, abort_addr, WQ_QFREE);
-            }
+            if (is_k && w.first && pieces > 0) ok = mbar_wait_lean(bar(PB_QFREE), (pieces - 1) & 1u, abort_addr, WQ_QFREE);
 #pragma unroll 1
             for (int n = g; n < 4 && ok; n += is_k ? 2 : 4) {
                 const int c0 = is_k ? 2 * n : 4 * (int)rank + 2 * (g & 1), c1 = is_k && n == 3 ? PP_CHUNKS : c0 + 2;
@@ -406,6 +401,9 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                 if (it >= 1) ok = mbar_wait_lean(bar(is_k ? PB_KFREE + n : PB_VFREE + h), (it - 1) & 1u, abort_addr, is_k ? WQ_KFREE : WQ_VFREE);
                 if (!ok) break;
                 if (elect_one()) {
+                    // Which rows are there: by the lane whose arrival hands it over.  (The slot's last readers, the softmax warps eight blocks
+                    // ago, gave their score buffer back long before.)
+                    if (is_k && n == 0) *reinterpret_cast<uint4*>(sm + PPY_OFF + 16 * (it & 7)) = make_uint4(w.valid[0], w.valid[1], w.valid[2], w.valid[3]);
                     mbar_arrive_expect_tx_remote(full, (uint32_t)(c1 - c0) * bytes);
                     if (half == 1 && e0 >= 0) {
 #pragma unroll 1

@@ -43,3 +43,19 @@ def test_waits_ask_for_a_phase_next_to_one_that_is_over():
     # nothing is read from the accumulator in the epilogue before all four warps have waited
     epilogue = body[body.rindex("mbar_wait_lean(bar(PB_VFREE + 1)"):]
     assert epilogue.index("named_bar_or(1 + grp, 128, dead)") < epilogue.index("tc_fence_after();") < epilogue.index("tmem_ld32(")
+
+
+def test_who_stores_which_rows_are_there_hands_it_over():
+    """The lane that stores a block's validity arrives on the barrier that makes it readable: either one elected lane does both, or lane 0
+    does, behind the warp's other stores."""
+    for name, at in (("paged.cu", "GV_OFF"), ("paged_pair.cu", "PPY_OFF")):
+        text = _source(name)
+        stores = [m.start() for m in re.finditer(r"\(sm \+ " + at + r"[^;]*\) = ", text)]
+        assert stores
+        for i in stores:
+            elected, lane0 = text.rfind("if (elect_one()) {", 0, i), text.rfind("if (lane == 0)", 0, i)
+            arrive = re.compile(r"mbar_arrive\w*\(").search(text, i).start()
+            if elected > lane0:
+                assert "}" not in text[elected:arrive], name
+            else:
+                assert "elect_one" not in text[i:arrive] and "if (lane == 0) mbar_arrive(" in text[i:arrive + 12], name

@@ -351,8 +351,9 @@ int smla_decode_splitkv_noalloc(const void* q, const void* kv, const int32_t* in
  *   slots      [num_tokens] int32, or int64 where slots64: row slots[t] of the cache (page slots[t] / page_block_size) takes token
  *              t; a slot outside [0, num_pages * page_block_size) leaves the cache as it is.  Slots differ from one another.
  *   positions  [num_tokens] int32 or int64, rows of cos_sin [num_positions, 64] fp32 (32 cosines | 32 sines); both NULL: nothing is
- *              rotated.  A token whose position lies outside the table leaves nothing, in no output.
- *   neighbours 1: values 2 i and 2 i + 1 turn by angle i; 0: values i and i + 32
+ *              rotated.  A token whose position lies outside the table leaves the cache, and its vectors of q_out, as they are.
+ *   neighbours bit 0: values 2 i and 2 i + 1 turn by angle i, else values i and i + 32; bit 1: zeros in q_out for a token whose position
+ *              lies outside the table
  *   q_pe       [num_tokens, num_heads, 64] -> q_out, both with distances between tokens and heads in values (NULL: no queries); q_out
  *              may be q_pe itself
  * All vectors start on 16 bytes, MODEL1 pages on 8, others on 16.
@@ -368,6 +369,7 @@ int smla_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_pe, int6
  * row of 128 are rotated as above (rope_offset 0 or 64), in fp32; then scale = max(|x|, 1e-4) / 448 and e4m3(x / scale).
  *   k [num_tokens, 128] bf16 (rows k_stride values apart) -> ki [capacity, 128] e4m3, k_scale [capacity] fp32, at slots[t] (as above)
  *   q [num_tokens, num_heads, 128] bf16 -> qi e4m3, w_out [num_tokens, num_heads] = weights * scale (weights NULL: the scale); q NULL: none
+ * A token whose position lies outside the table leaves no key, and zeros in qi and w_out.
  * No counterpart in the reference.
  */
 int smla_append_index(const void* k, int64_t k_stride, void* ki, float* k_scale, int64_t capacity, const void* slots, int slots64,

@@ -505,8 +505,8 @@ int smla_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_pe, int6
     p.slots = slots; p.slots64 = slots64; p.positions = positions; p.positions64 = positions64; p.cos_sin = cos_sin; p.num_positions = num_positions;
     if (num_heads > 0) { p.q_pe = (const uint16_t*)q_pe; p.q_out = (uint16_t*)q_out; }
     p.q_pe_token = q_pe_token; p.q_pe_head = q_pe_head; p.q_out_token = q_out_token; p.q_out_head = q_out_head;
-    p.num_tokens = num_tokens; p.num_heads = num_heads;
-    return launch_append_kv(p, layout, neighbours != 0, (cudaStream_t)stream);
+    p.num_tokens = num_tokens; p.num_heads = num_heads; p.clear_lost = (neighbours & 2) != 0;
+    return launch_append_kv(p, layout, (neighbours & 1) != 0, (cudaStream_t)stream);
 }
 
 int smla_append_index(const void* k, int64_t k_stride, void* ki, float* k_scale, int64_t capacity, const void* slots, int slots64,

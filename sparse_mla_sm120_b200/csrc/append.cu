@@ -95,7 +95,7 @@ template <int LAYOUT, bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) 
     // The values are asked for before the position, the table's entry and the slot are known: else a warp waits for memory two or three
     // times in a row (8192 tokens of 128 heads 64.1 -> 53.9 us).
     const int64_t pos = p.positions != nullptr ? ld_index(p.positions, p.positions64, t) : 0;
-    const bool lost = p.positions != nullptr && (pos < 0 || pos >= p.num_positions);       // a token without a position leaves nothing
+    const bool lost = p.positions != nullptr && (pos < 0 || pos >= p.num_positions);       // a token without a position leaves nothing, or zeros in q_out
     if (part > 0) {
         const uint16_t* src = p.q_pe + t * p.q_pe_token;
         uint16_t* dst = p.q_out + t * p.q_out_token;
@@ -104,7 +104,14 @@ template <int LAYOUT, bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) 
 #pragma unroll
         for (int i = 0; i < KV_HEADS / 4; ++i)
             if (h0 + 4 * i < p.num_heads) v[i] = ld_rot<PAIRS>(src + (h0 + 4 * i) * p.q_pe_head, l);
-        if (lost) return;
+        if (lost) {
+            if (p.clear_lost) {
+#pragma unroll
+                for (int i = 0; i < KV_HEADS / 4; ++i)
+                    if (h0 + 4 * i < p.num_heads) st_rot<PAIRS>(dst + (h0 + 4 * i) * p.q_out_head, l, make_uint4(0, 0, 0, 0));
+            }
+            return;
+        }
         c = ld_in(reinterpret_cast<const float4*>(p.cos_sin + pos * 64) + l);
         s = ld_in(reinterpret_cast<const float4*>(p.cos_sin + pos * 64 + 32) + l);
 #pragma unroll
@@ -219,7 +226,18 @@ template <bool PAIRS> __global__ void __launch_bounds__(WARPS * 32) append_index
     }
     int64_t slot = 0;
     if (part == 0) slot = ld_index(p.slots, p.slots64, t);
-    if (p.positions != nullptr && (pos < 0 || pos >= p.num_positions)) return;
+    if (p.positions != nullptr && (pos < 0 || pos >= p.num_positions)) {        // no key; queries of zeros and weight zero
+        if (part > 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = 2 * i + (lane >> 4);
+                if (r >= rows) break;
+                *reinterpret_cast<uint2*>(p.qi + (row0 + r) * 128 + l * 8) = make_uint2(0, 0);
+                if (l == 0) p.w_out[row0 + r] = 0.f;
+            }
+        }
+        return;
+    }
     // the rotated half of the row lies in eight neighbouring lanes
     const bool turns = p.positions != nullptr && (l >> 3) == (p.rope_offset >> 6);
     float c[8], s[8];

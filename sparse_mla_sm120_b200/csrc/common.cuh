@@ -163,7 +163,7 @@ struct AppendKvParams {
     const void* positions; int positions64;
     const float* cos_sin; int64_t num_positions;
     const uint16_t* q_pe; int64_t q_pe_token, q_pe_head;
-    uint16_t* q_out; int64_t q_out_token, q_out_head;
+    uint16_t* q_out; int64_t q_out_token, q_out_head; int clear_lost;    // clear_lost: zeros for tokens without a position
     int num_tokens, num_heads, parts;
 };
 struct AppendIndexParams {

@@ -560,8 +560,9 @@ PyObject* append_kv(const Args& x) {
     require_cuda({&kv_c, &k_pe, &kv, &at.slots, &at.positions, &at.cos_sin, &q_pe, &q_out});
     require_one_device(kv, {&kv_c, &k_pe, &at.slots, &at.positions, &at.cos_sin, &q_pe, &q_out});
     const c10::cuda::CUDAGuard on(kv.device());
-    if (q_pe.defined() && !q_out.defined()) q_out = at::empty({n, heads, 64}, q_pe.options());
-    const int pairs = (int)x.integer(6);
+    const bool own = q_pe.defined() && !q_out.defined();        // (its vectors of tokens without a position are zeros)
+    if (own) q_out = at::empty({n, heads, 64}, q_pe.options());
+    const int pairs = (x.integer(6) != 0 ? 1 : 0) | (own ? 2 : 0);
     launch([&] {
         const bool q = q_pe.defined() && q_pe.numel() > 0;
         return api.append_kv(ptr(kv_c), distance(kv_c, 0), ptr(k_pe), distance(k_pe, 0), ptr(kv), g.layout, g.pages, (int)g.block, g.stride,

@@ -25,7 +25,7 @@ def append_kv_cache(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tens
     gets pieces of either.
     ``positions`` [T] (int32 or int64) are rows of ``cos_sin`` [positions, 64] fp32, 32 cosines and 32 sines; without both nothing is
     rotated.  ``interleaved``: values 2i and 2i + 1 turn by angle i, else values i and i + 32.  A token whose position lies outside
-    the table leaves nothing, in the cache or in q_out.
+    the table leaves the cache and a given q_out as they are; an allocated q_out has zeros for it.
     ``q_pe`` [T, H, 64], the same tokens' queries, any distances between tokens and heads -> ``q_out`` (allocated if not given; a
     slice of the query [T, H, 576], or q_pe itself), which is returned."""
     return native().append_kv(kv_c, k_pe, kv_cache, slot_mapping, positions, cos_sin, interleaved, q_pe, q_out)
@@ -40,7 +40,7 @@ def append_indexer_keys(k: torch.Tensor, ki: torch.Tensor, k_scale: torch.Tensor
     rounded once, from fp32.  Slots, positions, cos_sin and interleaved as in append_kv_cache.
 
     With ``q`` [T, H, 128] bf16 the same tokens' queries too; returns (qi [T, H, 128] e4m3, weights [T, H] fp32 times each query's scale,
-    or the scales where no weights are given)."""
+    or the scales where no weights are given), zeros both for a token whose position lies outside the table."""
     return native().append_index(k, ki, k_scale, slot_mapping, positions, cos_sin, interleaved, rope_offset, q, weights)
 
 

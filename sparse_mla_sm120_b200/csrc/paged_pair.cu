@@ -190,8 +190,8 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
         const int col0 = 64 * thalf + 32 * ch;                    // the thread's rows of a block: [col0, + 32)
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
         // The sign of the softmax scale goes into the scores.  Never 0: rows that are not seen have scores of -inf, and -inf times 0 would be no
-        // number; 2^-62 times any score is far below one step of an exponent.  (A scale that is no number stays none.)
-        const float c = p.sm_scale == p.sm_scale ? fmaxf(fabsf(p.sm_scale * LOG2E), 0x1p-62f) : p.sm_scale;
+        // number; the smallest normal number takes scores of up to 2^100 to nothing.  (A scale that is no number stays none.)
+        const float c = p.sm_scale == p.sm_scale ? fmaxf(fabsf(p.sm_scale * LOG2E), 0x1p-126f) : p.sm_scale;
         const bool negative = p.sm_scale < 0.f;
         float* xch = reinterpret_cast<float*>(sm + PPX_OFF);
         const uint32_t s_free = barp(PB_SFREEP), p_ready = barp(PB_PREADYP + thalf);

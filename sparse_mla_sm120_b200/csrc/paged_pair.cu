@@ -269,10 +269,18 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
                     tc_fence_after();
                 }
                 const float mm = m == -INFINITY ? 0.f : -m;
+                // s c - m in one rounding is off from the rounded maximum by as much as that was rounded: harmless (it stands in all weights and in
+                // their sum) while that is less than a step of an exponent, but not where scores have steps of hundreds.
+                float cc = c;
+                if (fabsf(mm) >= 0x1p24f) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * c);
+                    cc = 1.f;
+                }
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float a = ex2(fmaf(__uint_as_float(sv[2 * i]), c, mm)), e = ex2(fmaf(__uint_as_float(sv[2 * i + 1]), c, mm));
+                    const float a = ex2(fmaf(__uint_as_float(sv[2 * i]), cc, mm)), e = ex2(fmaf(__uint_as_float(sv[2 * i + 1]), cc, mm));
                     l += a + e;
                     w[i] = pack_weights<F16>(a, e);
                 }

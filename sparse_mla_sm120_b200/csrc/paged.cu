@@ -265,7 +265,7 @@ attn_paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap q_map
             if (half == 0 && quad < 2) {                          // one lane for each of the quad's rows
                 const int r = quad == 0 ? ra : rb;
                 const float l = other[r] + other[PG_ROWS + r], m = quad == 0 ? m_a : m_b;
-                float lse = l == 0.f ? NEG_BIG : log2f(l) + m, denom = l;
+                float lse = l == 0.f ? (whole ? NEG_BIG : NO_RECORD) : log2f(l) + m, denom = l;
                 if (r < live) {
                     if (whole && p.attn_sink != nullptr) {
                         const float sink2 = ld_in(p.attn_sink + (row0 + r) % p.num_heads) * LOG2E;
@@ -609,12 +609,12 @@ template <bool F16, int W> __global__ void __launch_bounds__(combine_warps(W) * 
             }
     };
     load(warp);
-    float mx = NEG_BIG, sum = 0.f;
+    float mx = NO_RECORD, sum = 0.f;
     for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ld_in(p.lse_part + record(s)));
     mx = warp_max(mx);
     for (int s = lane; s < n; s += 32) {
         const float x = ld_in(p.lse_part + record(s));
-        sum += x == NEG_BIG ? 0.f : exp2f(x - mx);
+        sum += x == NO_RECORD ? 0.f : exp2f(x - mx);
     }
     sum = warp_sum(sum);
     float lse = sum == 0.f ? NEG_BIG : log2f(sum) + mx, denom = sum;
@@ -633,7 +633,7 @@ template <bool F16, int W> __global__ void __launch_bounds__(combine_warps(W) * 
         for (int u = 0; u < PC_AHEAD; ++u) {
             const int s = s0 + W * u;
             if (s >= n) break;
-            const float x = ld_in(p.lse_part + record(s)), w = x == NEG_BIG ? 0.f : exp2f(x - mx) * inv;
+            const float x = ld_in(p.lse_part + record(s)), w = x == NO_RECORD ? 0.f : exp2f(x - mx) * inv;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 acc[i].x += w * v[u][i].x; acc[i].y += w * v[u][i].y; acc[i].z += w * v[u][i].z; acc[i].w += w * v[u][i].w;

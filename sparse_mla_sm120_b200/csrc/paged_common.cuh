@@ -18,6 +18,7 @@ constexpr int PG_START = 2;
 // The running maximum of a row lags by at most 2^PG_TAU: weights are floating point, so that costs no precision (fp16 weights reach
 // 2^8 and fall to zero 2^-24 below a maximum that does not lag), and the accumulator is rescaled a few times per request.
 constexpr float PG_TAU = 8.0f;
+constexpr float NO_RECORD = -INFINITY;            // the LSE of a partition's record in which a query row sees nothing (scores may lie below NEG_BIG)
 constexpr uint32_t G_CHUNK = 64 * 128;            // 64 dims of 64 rows, 128B swizzle
 
 __device__ __forceinline__ uint32_t gswz(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }

@@ -326,7 +326,7 @@ attn_paged_pair_kernel(const PagedParams p, const __grid_constant__ CUtensorMap 
             l = (xch[hrow] + xch[64 + hrow]) + (xch[128 + hrow] + xch[192 + hrow]);
             const size_t rec = whole ? (size_t)piece.req : (size_t)(2 * part + (piece.b0 == 0 ? 1 : 0));
             const size_t row = rec * p.rows + row0 + hrow;
-            float lse = l == 0.f ? NEG_BIG : log2f(l) + m, denom = l;
+            float lse = l == 0.f ? (whole ? NEG_BIG : NO_RECORD) : log2f(l) + m, denom = l;
             if (whole && p.attn_sink != nullptr && hrow < live) {
                 const float sink2 = ld_in(p.attn_sink + (row0 + hrow) % p.num_heads) * LOG2E;
                 if (l != 0.f) denom += exp2f(sink2 - m);

@@ -47,3 +47,22 @@ def test_scores_whose_own_roundings_are_large(kind, heads, size):
         w = P.HALF_STEP[q.dtype]
         assert bool(((out[b, 0].cpu().double() - v).abs() <= (2 * w + w * w + 2.0 ** -21) * v.abs() + 2.0 ** -24)[sure].all())
         assert bool(((lse[b, 0].cpu().double() - top[:, 0] * 1.4426950408889634).abs() <= 1.45 * off + 2.0 ** -22 * top[:, 0].abs())[sure].all())
+
+
+@pytest.mark.parametrize("heads", [16, 96])
+@pytest.mark.parametrize("parts", [1, 2, 5, None])
+@pytest.mark.parametrize("sink", [False, True])
+def test_scores_far_below_what_stands_for_nothing(heads, parts, sink):
+    """Scores of some -5e32, below the -1e30 that the LSE of a row without anything has: all rows alike, so the output is the row."""
+    q, cache, table, n, scale = _case("bf16", [700, 130, 0], 1, heads, 64, 9)
+    row = torch.where(torch.arange(576, device=DEV) % 3 == 0, -2.0 ** 53, 2.0 ** 52).to(torch.bfloat16)
+    cache[:] = row
+    q[:] = -row
+    sinks = torch.full((heads,), float("-inf"), device=DEV) if sink else None
+    out, lse = _run(q, cache, table, n, scale, num_sm_parts=parts, attn_sink=sinks)
+    s = float((row.double() * -row.double()).sum()) * scale * 1.4426950408889634
+    # equal weights of 1, whole numbers of them: exact sums but for the merge's products, the division and the output's rounding
+    assert s < -1e32
+    assert float((out[:2].double() - row[:512].double()).abs().max()) <= (2.0 ** -8 + 700 * 2.0 ** -23) * 2.0 ** 53
+    assert float((lse[:2].double() - s).abs().max()) <= 576 * 2.0 ** -23 * -s
+    assert bool((out[2] == 0).all()) and bool((lse[2] == -1e30).all())

@@ -355,7 +355,7 @@ int smla_decode_splitkv_noalloc(const void* q, const void* kv, const int32_t* in
  *   neighbours bit 0: values 2 i and 2 i + 1 turn by angle i, else values i and i + 32; bit 1: zeros in q_out for a token whose position
  *              lies outside the table
  *   q_pe       [num_tokens, num_heads, 64] -> q_out, both with distances between tokens and heads in values (NULL: no queries); q_out
- *              may be q_pe itself
+ *              may be q_pe itself; its vectors do not overlap
  * All vectors start on 16 bytes, MODEL1 pages on 8, others on 16.
  */
 int smla_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_pe, int64_t k_pe_stride, void* cache, int layout,

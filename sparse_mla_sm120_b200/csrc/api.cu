@@ -499,6 +499,13 @@ int smla_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_pe, int6
     if (!aligned16(kv_c) || !aligned16(k_pe) || !aligned16(q_pe) || !aligned16(q_out) ||
         ((kv_c_stride | k_pe_stride | (q_pe ? q_pe_token | q_pe_head | q_out_token | q_out_head : 0)) & 7))
         return set_error(SMLA_E_ALIGN, "%s: every vector must start on 16 bytes", fn);
+    if (q_out != nullptr) {        // two vectors in one place would be written by two warps
+        const bool tokens_inside = num_heads > 1 && (num_tokens <= 1 || q_out_token < q_out_head);
+        const int64_t near = tokens_inside ? q_out_token : q_out_head, far = tokens_inside ? q_out_head : q_out_token;
+        const int n_near = tokens_inside ? num_tokens : num_heads, n_far = tokens_inside ? num_heads : num_tokens;
+        const int64_t extent = n_near > 1 ? (int64_t)(n_near - 1) * near + 64 : 64;
+        if ((n_near > 1 && near < 64) || (n_far > 1 && far < extent)) return set_error(SMLA_E_SHAPE, "%s: vectors of q_out overlap", fn);
+    }
     AppendKvParams p{};
     p.kv_c = (const uint16_t*)kv_c; p.kv_c_token = kv_c_stride; p.k_pe = (const uint16_t*)k_pe; p.k_pe_token = k_pe_stride;
     p.cache = (uint8_t*)cache; p.page_stride = page_stride_bytes; p.page_block_size = page_block_size; p.capacity = num_pages * page_block_size;

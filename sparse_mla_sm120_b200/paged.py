@@ -27,7 +27,7 @@ def append_kv_cache(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tens
     rotated.  ``interleaved``: values 2i and 2i + 1 turn by angle i, else values i and i + 32.  A token whose position lies outside
     the table leaves the cache and a given q_out as they are; an allocated q_out has zeros for it.
     ``q_pe`` [T, H, 64], the same tokens' queries, any distances between tokens and heads -> ``q_out`` (allocated if not given; a
-    slice of the query [T, H, 576], or q_pe itself), which is returned."""
+    slice of the query [T, H, 576], or q_pe itself; no two vectors in one place), which is returned."""
     return native().append_kv(kv_c, k_pe, kv_cache, slot_mapping, positions, cos_sin, interleaved, q_pe, q_out)
 
 

@@ -379,7 +379,8 @@ int smla_append_index(const void* k, int64_t k_stride, void* ki, float* k_scale,
 
 /*
  * Attention of the newest query_len tokens of every request over all of the request's rows, found through a block table: split over the
- * rows, joined by a second kernel.  Products of the cache's values as bf16 (exact for the packed layouts) or fp16, sums and softmax in
+ * rows, joined by a second kernel.  Products of the cache's values as bf16 (of the packed layouts exact where scales are powers of two, as
+ * the writers make them, else rounded to it) or fp16, sums and softmax in
  * fp32, weights rounded to the 16-bit type for their product with V.  The reference takes block_table and cache_seqlens in this place and
  * serves index lists only (flash_mla_sm120/interface.py:39-58).
  *   q           [batch, query_len, num_heads, 576 (512 for MODEL1)] bf16 (fp16 for SMLA_LAYOUT_F16), contiguous
@@ -389,6 +390,7 @@ int smla_append_index(const void* k, int64_t k_stride, void* ki, float* k_scale,
  *   causal      1: query i sees the rows [0, length - query_len + 1 + i); 0: all
  *   attn_sink   [num_heads] fp32 natural-log or NULL
  *   out         [batch, query_len, num_heads, 512], lse the same without 512: base 2 with the sink in it, 0 and -1e30 where nothing is seen
+ *               (with a sink above -inf: 0 and the sink)
  *   num_parts   partitions that the rows of all requests are cut into (0: one per SM and 64 query rows)
  *   scratch     smla_paged_scratch_bytes(...) bytes
  */

@@ -20,15 +20,17 @@
 // Every wait is bounded; a wait that gives up records a code in status[] and the CTA drains and exits.
 //
 // Which calls come here: up to 64 query rows per request, and packed rows; more query rows of 16-bit caches go to paged_pair.cu (64
-// requests of up to 8192 rows, 128 heads: 149.6 us here with every row read by two CTAs, 116.2 there).
+// requests of up to 8192 rows, 128 heads: 149.6 us here with every row read by two CTAs, 114 to 118 there).
 // What bounds it: with few query rows the products, whose operands of 64 rows make shared memory the limit (36 + 16 products of a block: 2300
 // cycles for 16 query rows as for 64), of a block's 2700 to 3100; a call of a few blocks is a chain of latencies (entry, lengths, table, rows,
 // four blocks, epilogue, merge: 13.8 us for 1000 rows).  Packed rows: the way through registers, about 5000 cycles for a warp's 16 rows.
 // 48 requests of up to 4096 fp16 rows in pages of 16, two tokens of 16 heads: 44.5 us, 2.9 TB/s; 656-byte rows, 64 requests of up to 8192, 64
-// heads: 102 us; 584-byte, 13 of up to 16384, 128 heads: 91.9 us.
+// heads: 102 us; 584-byte, 13 of up to 16384, 128 heads: 92.5 us.  Of a prompt's chunk under a causal mask all blocks are walked, also those that
+// no query row of the CTA sees (256 tokens of 16 heads over 4096 rows: bf16 54 us, 656-byte 126).
 // What the steps brought (the first version, rows by one warp and one stage of waiting: 52.5, 122.8, 104.7 us): rows by TMA from four warps and
 // stages in quarters 49.1, 118.9, 94.0; rows asked into L2 ahead and a shorter epilogue 44.6, 116.8, 96.8; fewer registers spilled (a spilled
-// register costs hundreds of cycles beside 220 KB of shared memory) and packed rows asked into L2 ahead 44.5, 101.9, 91.9.  Measured and not
+// register costs hundreds of cycles beside 220 KB of shared memory) and packed rows asked into L2 ahead 44.5, 101.9, 91.9;
+// hidden rows judged by their values 44.5, 101.8, 92.6.  Measured and not
 // kept: a packed row's values asked for as soon as those of the block before are in the stage (160, 110: the fence before a stage is handed over
 // waits for the loads).
 #include "paged_common.cuh"

@@ -15,9 +15,9 @@
 //
 // What bounds it: memory and the chain K -> scores -> softmax -> P.V about equally, 3900 to 4300 cycles per block (136 KB per CTA from L2, 147 KB per
 // pair from HBM: 5 TB/s), and what a request costs besides: 15000 cycles before the first scores, 9000 for an epilogue.
-// 64 requests of up to 8192 rows, 128 heads: 116.2 us (3.1 TB/s, 707 TFLOP/s); one of 131072: 58.5 us, of which the merge takes 9.
+// 64 requests of up to 8192 rows, 128 heads: 114 to 118 us from one B200 to another (3.0 TB/s, 700 TFLOP/s); one of 131072: 58 us, of which the merge takes 9.
 // The steps (us, both cases): as two CTAs of paged.cu 149.6, 72.7; first version 129.9, 65.8; the even CTA's barriers take the bytes of both,
-// weights handed over by halves, epilogue through shared memory, no spilled registers (16 warps of 128 registers) 116.4, 60.1.  Measured and not
+// weights handed over by halves, epilogue through shared memory, 16 warps of 128 registers (16 bytes of them spilled) 116.4, 60.1.  Measured and not
 // kept: a barrier per chunk of K (400 cycles each to issue: 135.4), V by two warps (141.5), 20 warps that trade registers (131.1).
 //
 // Warps: 0-7 softmax and epilogue (thread = one query row x 32 rows of a block), 8 and 9 bring in K and the queries, 10-13 V (64 rows x

@@ -20,7 +20,8 @@ def append_kv_cache(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tens
     turned by the token's angles.  Both may be slices of one projection's output (rows any multiple of 8 values apart).
 
     ``kv_cache``: 656-byte rows, 584-byte pages, or [num_blocks, block, 1, 576] bf16 / fp16, whose type kv_c, k_pe and the queries
-    have (bf16 for the byte layouts); pages may be padded.  Slots (int32 or int64) number rows through the pages: page s // block, row
+    have (bf16 for the byte layouts); pages may be padded, and start on 16 bytes (584-byte pages on 8: those of an odd number of rows can be
+    written without padding, but not read by paged_mla_decode_fwd).  Slots (int32 or int64) number rows through the pages: page s // block, row
     s % block.  One outside the cache, -1 say, leaves the cache as it is.  Slots must differ: of two tokens with one slot the row
     gets pieces of either.
     ``positions`` [T] (int32 or int64) are rows of ``cos_sin`` [positions, 64] fp32, 32 cosines and 32 sines; without both nothing is
@@ -50,11 +51,15 @@ def paged_mla_decode_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     """Attention of the newest tokens over all rows of their request: attention split over the rows -> merge.
 
     ``q`` [B, s_q, H, 576] or [B, H, 576] (512 wide over 584-byte pages), bf16 (fp16 over fp16 rows), H up to 128; ``kv_cache``
-    [num_blocks, block, 1, 576] bf16 / fp16, or the 656- and 584-byte layouts; ``block_table`` [B, pages] int32 (rows any distance apart);
+    [num_blocks, block, 1, 576] bf16 / fp16, or the 656- and 584-byte layouts, pages on 16 bytes (584-byte pages of an odd number of rows
+    therefore padded); ``block_table`` [B, pages] int32 (rows any distance apart);
     ``cache_seqlens`` [B] int32 rows of each request, the new tokens' own among them (0: none; more than the table has pages for: all of
     those).  ``causal``: query i of s_q sees rows [0, cache_seqlens - s_q + 1 + i).  Rows in pages that the cache does not have (-1, say)
     count as no entry.  ``num_sm_parts``: partitions that all rows are cut into (default: one per SM and 64 query rows).
-    Returns (out [..., H, 512] in q's type, lse [..., H] fp32, base 2 with the sink in it); 0 and -1e30 where a query sees nothing.
+    Returns (out [..., H, 512] in q's type, lse [..., H] fp32, base 2 with the sink in it); 0 and -1e30 where a query sees nothing (with a
+    sink above -inf: 0 and the sink).  What a query does not see has no part in its output, NaN and infinities included, in rows or in other
+    queries.  (An infinity in a row that a query does see and scores at minus infinity: 0 times infinity is no number; but in the newest
+    s_q - 1 rows under a causal mask, which other queries must not see, it may count as nothing.)
     Exact numerics: products of 16-bit values (the byte layouts' are exact in bf16 where their scales are
     powers of two, as append_kv_cache and pack_kv_cache write them, else rounded to it), fp32 sums and softmax; weights are rounded to 16
     bits for their product with V."""
